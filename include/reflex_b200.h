@@ -61,7 +61,7 @@ int rfx_abi_version(void);
 /* sizeof() of the args struct with the given index (0 RfxKvAppendArgs, 1 RfxKvLookupArgs,
  * 2 RfxRopeArgs, 3 RfxRopeTableArgs, 4 RfxRopeAppendArgs, 5 RfxSoftmaxArgs,
  * 6 RfxAttentionArgs, 7 RfxPagedAttentionArgs, 8 RfxCombineArgs, 9 RfxHeadGatherArgs,
- * 10 RfxPeerHandle, 11 RfxLinearNormArgs; 0 for anything else), so
+ * 10 RfxPeerHandle, 11 RfxLinearNormArgs, 12 RfxQkNormRopeArgs; 0 for anything else), so
  * a foreign-function binding can verify its struct mirrors before the first call. */
 size_t rfx_args_size(int which);
 const char* rfx_status_string(int status);
@@ -189,6 +189,47 @@ typedef struct {
     float* v_scales;
 } RfxRopeAppendArgs;
 int rfx_rope_append(const RfxRopeAppendArgs* a);
+
+/* RMS norm of every query and key head, then the rotation of the normed head, in one pass (models that
+ * norm Q and K per head; no counterpart in the reference, whose norm and rotation are separate calls):
+ *   n = x / sqrt(mean(x^2) + eps) * weight;   y = rotation of n by table row positions[token]
+ * in fp32 with one rounding at the end. The tables are [table_rows, D] in `dtype` or (tables_f32) fp32;
+ * of a row the first half (interleaved: the even entries) is read, as in rfx_rope_apply.
+ * rfx_qk_norm_rope writes dense rows q_out and k_out (each may be its input, strides included); a token
+ * whose position has no table row gives zeros, or is left as it is where it is rotated in place.
+ * rfx_qk_norm_rope_append writes Q to q_out, the normed and rotated K and the plain V to the pool at
+ * slot_mapping; a token without a table row leaves the pool as it is (its q_out row as above), one whose
+ * slot lies outside the pool is skipped there. int8 pool: rows are quantised from the unrounded fp32
+ * values (see the layout note at the top). head_dim is even and at most 512. */
+typedef struct {
+    const void* q;               /* [N, H_q, D], strides below, last dim contiguous */
+    const void* k;               /* [N, H_kv, D] */
+    const void* v;               /* [N, H_kv, D]; append only */
+    void* q_out;
+    void* k_out;                 /* not for append */
+    void* k_cache;               /* append only: [num_blocks, H_kv, block_size, D] */
+    void* v_cache;
+    const int64_t* slot_mapping; /* [N]; append only */
+    const int32_t* positions;    /* [N]; NULL (not for append): token n has table row n */
+    const void* cos;             /* [table_rows, D], row stride table_stride */
+    const void* sin;
+    const void* q_weight;        /* [D] in dtype */
+    const void* k_weight;        /* [D] */
+    int64_t n_tokens, num_q_heads, num_kv_heads, head_dim, num_blocks, block_size, table_rows;
+    int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+    int64_t q_out_stride_n, q_out_stride_h, k_out_stride_n, k_out_stride_h;
+    int64_t cache_stride_blk, cache_stride_h, cache_stride_pos, table_stride;
+    float eps;
+    int interleaved;
+    int tables_f32;
+    int dtype;
+    int kv_int8;                 /* append only; caches int8 and contiguous, the cache strides are ignored */
+    float* k_scales;             /* [num_blocks, H_kv, block_size] */
+    float* v_scales;
+    rfx_stream stream;
+} RfxQkNormRopeArgs;
+int rfx_qk_norm_rope(const RfxQkNormRopeArgs* a);
+int rfx_qk_norm_rope_append(const RfxQkNormRopeArgs* a);
 
 /* ------------------------------------------------------------------ softmax ---- */
 

@@ -140,6 +140,7 @@ size_t rfx_args_size(int which) {
         case 9: return sizeof(RfxHeadGatherArgs);
         case 10: return sizeof(RfxPeerHandle);
         case 11: return sizeof(RfxLinearNormArgs);
+        case 12: return sizeof(RfxQkNormRopeArgs);
         default: return 0;
     }
 }

@@ -89,6 +89,21 @@ class RopeAppendArgs(C.Structure):
     ]
 
 
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("q_out", vp), ("k_out", vp), ("k_cache", vp), ("v_cache", vp),
+        ("slot_mapping", vp), ("positions", vp), ("cos", vp), ("sin", vp), ("q_weight", vp), ("k_weight", vp),
+        ("n_tokens", i64), ("num_q_heads", i64), ("num_kv_heads", i64), ("head_dim", i64), ("num_blocks", i64),
+        ("block_size", i64), ("table_rows", i64),
+        ("q_stride_n", i64), ("q_stride_h", i64), ("k_stride_n", i64), ("k_stride_h", i64),
+        ("v_stride_n", i64), ("v_stride_h", i64),
+        ("q_out_stride_n", i64), ("q_out_stride_h", i64), ("k_out_stride_n", i64), ("k_out_stride_h", i64),
+        ("cache_stride_blk", i64), ("cache_stride_h", i64), ("cache_stride_pos", i64), ("table_stride", i64),
+        ("eps", C.c_float), ("interleaved", C.c_int), ("tables_f32", C.c_int), ("dtype", C.c_int),
+        ("kv_int8", C.c_int), ("k_scales", vp), ("v_scales", vp), ("stream", vp),
+    ]
+
+
 class SoftmaxArgs(C.Structure):
     _fields_ = [
         ("x", vp), ("y", vp), ("rows", i64), ("n", i64),
@@ -166,6 +181,8 @@ EXPORTS = {
     "rfx_rope_apply": (C.c_int, [C.POINTER(RopeArgs)]),
     "rfx_rope_build_tables": (C.c_int, [C.POINTER(RopeTableArgs)]),
     "rfx_rope_append": (C.c_int, [C.POINTER(RopeAppendArgs)]),
+    "rfx_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRopeArgs)]),
+    "rfx_qk_norm_rope_append": (C.c_int, [C.POINTER(QkNormRopeArgs)]),
     "rfx_online_softmax": (C.c_int, [C.POINTER(SoftmaxArgs)]),
     "rfx_fused_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),
     "rfx_fused_attention": (C.c_int, [C.POINTER(AttentionArgs)]),
@@ -194,7 +211,8 @@ EXPORTS = {
 
 # Index of each mirror in rfx_args_size().
 ARG_STRUCTS = [KvAppendArgs, KvLookupArgs, RopeArgs, RopeTableArgs, RopeAppendArgs, SoftmaxArgs,
-               AttentionArgs, PagedAttentionArgs, CombineArgs, HeadGatherArgs, PeerHandle, LinearNormArgs]
+               AttentionArgs, PagedAttentionArgs, CombineArgs, HeadGatherArgs, PeerHandle, LinearNormArgs,
+               QkNormRopeArgs]
 
 
 def library_path() -> Path:
@@ -278,6 +296,9 @@ def check(status: int) -> None:
 def call(name: str, args: C.Structure, dev: torch.device) -> None:
     """Invoke an ``int f(const Args*)`` entry point with ``dev`` current."""
     fn = getattr(lib(), name)
+    if dev.index == torch.cuda.current_device():
+        check(fn(C.byref(args)))
+        return
     with torch.cuda.device(dev):
         check(fn(C.byref(args)))
 

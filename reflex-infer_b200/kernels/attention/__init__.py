@@ -7,6 +7,7 @@ Dense:
 
 Paged (additive; none of them changes the functions above):
     ``rope_append``        RoPE on new K (and optionally Q) + write K, V into the pool
+    ``qk_norm_rope_append``  the same with an RMS norm of every query and key head before the rotation
     ``paged_attention``    split-K attention straight from the pool, ragged query chunks,
                            bottom-right causal, optional RoPE fused into the Q load
     ``paged_decode``       the one-row-per-request case of ``paged_attention``
@@ -29,6 +30,7 @@ from typing import Optional
 import torch
 
 from .. import _native as N
+from ..rope import _norm_args
 
 
 def _resolve_head_repeat(num_heads_q: int, num_heads_kv: int) -> int:
@@ -472,6 +474,95 @@ def rope_append(
                           interleaved=interleaved, k_scales=k_scales, v_scales=v_scales).run()
 
 
+def qk_norm_rope_append(
+    q: Optional[torch.Tensor],
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    positions: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    *,
+    eps: float = 1e-6,
+    q_out: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
+) -> Optional[torch.Tensor]:
+    """``kernels.rope.qk_norm_rope`` of ``q`` and ``k_new`` and the append of K and V to the pool, in one
+    launch. Returns the normed and rotated queries (``q_out``, which may be ``q``).
+
+    ``q``: ``[N, H_q, D]`` (or ``None``: K and V only, returns ``None``), ``k_new``/``v_new``:
+    ``[N, H_kv, D]``, any token and head strides; the pool as in ``rope_append``, tables and weights as in
+    ``qk_norm_rope``. fp32 throughout, one rounding (16- and 32-bit pools); an int8 pool takes
+    ``scale = max|row| / 127``, ``q = round(row / scale)`` of the unrounded rows. Slots must be distinct; a
+    slot outside the pool is skipped. A token whose position lies outside the tables leaves the pool as it
+    is; its row of ``q_out`` is zero, or unchanged if ``q_out`` is ``q``.
+    """
+    name = "qk_norm_rope_append"
+    dev = N.require_cuda(name, q, k_new, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin, q_weight,
+                         k_weight, q_out, k_scales, v_scales)
+    if k_new.stride(-1) != 1:
+        k_new = k_new.contiguous()
+    if v_new.stride(-1) != 1:
+        v_new = v_new.contiguous()
+    if q is not None and q.stride(-1) != 1:
+        q = q.contiguous()
+    if positions is None:
+        raise ValueError(f"{name}: positions are required")
+    a, keep = _norm_args(name, q, k_new, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    n, hkv, D = k_new.shape
+    if v_new.shape != k_new.shape or v_new.dtype != k_new.dtype:
+        raise ValueError(f"{name}: v_new must be like k_new, {tuple(k_new.shape)} in {k_new.dtype}")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride():
+        raise ValueError(f"{name}: caches must both be [num_blocks, H_kv, block_size, D] with one stride pattern")
+    nb, ch, bs, cd = k_cache.shape
+    if (hkv, D) != (ch, cd):
+        raise ValueError(f"{name}: input heads/head_dim {(hkv, D)} do not match the cache {(ch, cd)}")
+    kv_int8 = k_cache.dtype == torch.int8
+    if kv_int8:
+        if v_cache.dtype != torch.int8 or k_scales is None or v_scales is None:
+            raise ValueError(f"{name}: an int8 pool needs int8 k_cache and v_cache and k_scales, v_scales")
+        if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            raise ValueError(f"{name}: an int8 pool must be contiguous")
+        for t in (k_scales, v_scales):
+            if t.dtype != torch.float32 or tuple(t.shape) != (nb, ch, bs) or not t.is_contiguous():
+                raise ValueError(f"{name}: scales must be contiguous float32 [{nb}, {ch}, {bs}]")
+        a.kv_int8, a.k_scales, a.v_scales = 1, k_scales.data_ptr(), v_scales.data_ptr()
+    elif k_cache.dtype != k_new.dtype or v_cache.dtype != k_new.dtype:
+        raise RuntimeError(f"{name}: input dtype {k_new.dtype} does not match cache dtype {k_cache.dtype}")
+    if k_cache.stride(3) != 1:
+        raise ValueError(f"{name}: the head_dim axis of the caches must be contiguous")
+    if slot_mapping.shape != (n,):
+        raise ValueError(f"{name}: slot_mapping must be [N]={n}, got {tuple(slot_mapping.shape)}")
+    if slot_mapping.dtype != torch.int64:
+        slot_mapping = slot_mapping.to(torch.int64)
+    slot_mapping = slot_mapping.contiguous()
+    if q is None:
+        q_out = None
+    else:
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(-1) != 1:
+            raise ValueError(f"{name}: q_out must be shaped like q, in its dtype, with a contiguous last axis")
+        elif any(st == 0 and size > 1 for st, size in zip(q_out.stride(), q_out.shape)):
+            raise ValueError(f"{name}: q_out must not be an expanded view")
+        a.q_out = q_out.data_ptr()
+        a.q_out_stride_n, a.q_out_stride_h, _ = q_out.stride()
+    a.v, a.k_cache, a.v_cache, a.slot_mapping = (v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                 slot_mapping.data_ptr())
+    a.v_stride_n, a.v_stride_h, _ = v_new.stride()
+    a.num_blocks, a.block_size = nb, bs
+    a.cache_stride_blk, a.cache_stride_h, a.cache_stride_pos, _ = k_cache.stride()
+    a.stream = N.stream_handle(dev)
+    N.call("rfx_qk_norm_rope_append", a, dev)
+    return q_out
+
+
 def int8_pool(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int, device):
     """An empty int8 KV pool: ``(k_cache, v_cache, k_scales, v_scales)``, caches
     ``[num_blocks, H_kv, block_size, D]`` int8, scales ``[num_blocks, H_kv, block_size]`` float32."""
@@ -499,12 +590,24 @@ def paged_decode_step(
     out: Optional[torch.Tensor] = None,
     k_scales: Optional[torch.Tensor] = None,
     v_scales: Optional[torch.Tensor] = None,
+    q_norm_weight: Optional[torch.Tensor] = None,
+    k_norm_weight: Optional[torch.Tensor] = None,
+    norm_eps: float = 1e-6,
     **kw,
 ) -> torch.Tensor:
     """One decode step of one layer: append the new token's rotated K and its V to the
     pool, then attend the rotated query over ``context_lens`` keys (which count the new
     token). Three launches on top of the plan: RoPE+append, split-K partials with RoPE
-    fused into the Q load, combine."""
+    fused into the Q load, combine. With ``q_norm_weight`` and ``k_norm_weight`` (``[D]``) every query
+    and key head is RMS-normed before its rotation (``qk_norm_rope_append``, which then rotates Q too)."""
+    if (q_norm_weight is None) != (k_norm_weight is None):
+        raise ValueError("paged_decode_step: q_norm_weight and k_norm_weight go together")
+    if q_norm_weight is not None:
+        q_new = qk_norm_rope_append(q_new, k_new, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin,
+                                    q_norm_weight, k_norm_weight, eps=norm_eps, interleaved=interleaved,
+                                    k_scales=k_scales, v_scales=v_scales)
+        return paged_decode(q_new, k_cache, v_cache, block_table, context_lens, sm_scale=sm_scale,
+                            workspace=workspace, out=out, k_scales=k_scales, v_scales=v_scales, **kw)
     rope_append(k_new, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin, interleaved=interleaved,
                 k_scales=k_scales, v_scales=v_scales)
     return paged_decode(q_new, k_cache, v_cache, block_table, context_lens, sm_scale=sm_scale,
@@ -537,6 +640,7 @@ __all__ = [
     "paged_decode",
     "paged_decode_step",
     "rope_append",
+    "qk_norm_rope_append",
     "splitk_combine",
     "int8_pool",
     "PagedWorkspace",

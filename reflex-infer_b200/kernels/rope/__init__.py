@@ -6,6 +6,9 @@ reference's torch path: each multiply / add is rounded to the activation dtype
 (``kernels/rope/triton_rope.py:230-240``), so 16-bit outputs match it bit for bit when
 the tables carry the activation dtype (the way every reference test builds them,
 ``tests/test_rope.py:25-27``).
+
+``qk_norm_rope`` / ``qk_norm_rope_`` (additive) norm every query and key head before they rotate it,
+in one pass and in fp32 with a single rounding.
 """
 from __future__ import annotations
 
@@ -148,6 +151,127 @@ def build_rope_tables(
     return cos, sin
 
 
+def _norm_args(name, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    """The checks and fields that the dense form and the append share. Returns the args struct, the
+    device and the tensors that have to outlive the call. ``q`` may be ``None`` (no query heads)."""
+    if k.dim() != 3 or (q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2])):
+        raise ValueError(f"{name}: q must be [N, H_q, D] and k [N, H_kv, D]; "
+                         f"got {None if q is None else tuple(q.shape)} and {tuple(k.shape)}")
+    n, hkv, D = k.shape
+    if D % 2 != 0:
+        raise ValueError("head_dim must be even for RoPE")
+    dtype = k.dtype
+    code = N.dtype_code(k)
+    if q is not None and q.dtype != dtype:
+        raise RuntimeError(f"{name}: q dtype {q.dtype} differs from k dtype {dtype}")
+    for w in (q_weight, k_weight):
+        if w.shape != (D,):
+            raise ValueError(f"{name}: weights must be [{D}], got {tuple(w.shape)}")
+        if w.dtype != dtype:
+            raise RuntimeError(f"{name}: weight dtype {w.dtype} differs from the activations' {dtype}")
+    if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape:
+        raise ValueError(f"{name}: cos/sin must both be [rows, {D}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.dtype != sin.dtype or cos.dtype not in (dtype, torch.float32):
+        cos, sin = cos.to(dtype), sin.to(dtype)
+    if cos.stride(1) != 1 or sin.stride() != cos.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    if positions is not None:
+        if positions.shape != (n,):
+            raise ValueError(f"{name}: positions must be [N]={n}, got {tuple(positions.shape)}")
+        if positions.dtype != torch.int32:
+            positions = positions.to(torch.int32)
+        positions = positions.contiguous()
+    elif n > cos.shape[0]:
+        raise ValueError(f"{name}: {n} tokens without positions need as many table rows, got {cos.shape[0]}")
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError(f"{name}: eps must not be negative, got {eps}")
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    a = N.QkNormRopeArgs()
+    a.k, a.cos, a.sin = k.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    a.q_weight, a.k_weight, a.positions = q_weight.data_ptr(), k_weight.data_ptr(), N.ptr(positions)
+    a.n_tokens, a.num_kv_heads, a.head_dim = n, hkv, D
+    a.k_stride_n, a.k_stride_h, _ = k.stride()
+    if q is not None:
+        a.q, a.num_q_heads = q.data_ptr(), q.shape[1]
+        a.q_stride_n, a.q_stride_h, _ = q.stride()
+    a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
+    a.eps, a.interleaved = eps, int(bool(interleaved))
+    a.tables_f32, a.dtype = int(cos.dtype == torch.float32), code
+    return a, (cos, sin, positions, q_weight, k_weight)
+
+
+def _norm_rope(name, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    dev = N.require_cuda(name, q, k, q_weight, k_weight, cos, sin, positions)
+    a, keep = _norm_args(name, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
+    a.q_out_stride_n, a.q_out_stride_h, _ = q_out.stride()
+    a.k_out_stride_n, a.k_out_stride_h, _ = k_out.stride()
+    a.stream = N.stream_handle(dev)
+    N.call("rfx_qk_norm_rope", a, dev)
+    return q_out, k_out
+
+
+def qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    *,
+    positions: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    backend: Optional[str] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of ``q`` and ``k``, then its rotation; returns new contiguous tensors.
+
+    ``q``: ``[N, H_q, D]``, ``k``: ``[N, H_kv, D]``, any token and head strides (views of a packed
+    projection are read in place); ``q_weight``/``k_weight``: ``[D]`` in the activations' dtype;
+    ``cos``/``sin``: ``[rows, D]`` in float32 or the activations' dtype (others are cast to the latter);
+    ``positions``: ``[N]`` table row of each token (default: token ``n`` has row ``n``). ``D`` is even and
+    at most 512. A head is ``x / sqrt(mean(x^2) + eps) * weight``, rotated in pairs ``(i, i + D/2)`` or
+    (``interleaved``) ``(2i, 2i + 1)``; all in fp32, rounded once. A token whose position lies outside
+    the tables gives zeros.
+    """
+    N.check_backend(backend)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if k.stride(-1) != 1:
+        k = k.contiguous()
+    return _norm_rope("qk_norm_rope", q, k, None, None, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+def qk_norm_rope_(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    *,
+    positions: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    backend: Optional[str] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``qk_norm_rope`` in place; returns ``(q, k)``. The last axis of both must be contiguous and their
+    rows distinct memory (no expanded views). A token whose position lies outside the tables is left as
+    it is."""
+    N.check_backend(backend)
+    for t in (q, k):
+        if t.stride(-1) != 1:
+            raise ValueError("qk_norm_rope_: the head_dim axis must be contiguous to work in place")
+        if any(st == 0 and size > 1 for st, size in zip(t.stride(), t.shape)):
+            raise ValueError("qk_norm_rope_: an expanded view has no rows of its own to work in place")
+    return _norm_rope("qk_norm_rope_", q, k, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+
+
+# The reference's surface; qk_norm_rope and qk_norm_rope_ are additions, imported by name.
 __all__ = [
     "apply_rope",
     "apply_rope_",
