@@ -61,7 +61,8 @@ int rfx_abi_version(void);
 /* sizeof() of the args struct with the given index (0 RfxKvAppendArgs, 1 RfxKvLookupArgs,
  * 2 RfxRopeArgs, 3 RfxRopeTableArgs, 4 RfxRopeAppendArgs, 5 RfxSoftmaxArgs,
  * 6 RfxAttentionArgs, 7 RfxPagedAttentionArgs, 8 RfxCombineArgs, 9 RfxHeadGatherArgs,
- * 10 RfxPeerHandle, 11 RfxLinearNormArgs, 12 RfxQkNormRopeArgs; 0 for anything else), so
+ * 10 RfxPeerHandle, 11 RfxLinearNormArgs, 12 RfxQkNormRopeArgs,
+ * 13 RfxKvForkArgs, 14 RfxKvFreeArgs, 15 RfxKvCompactArgs, 16 RfxKvCopyArgs; 0 for anything else), so
  * a foreign-function binding can verify its struct mirrors before the first call. */
 size_t rfx_args_size(int which);
 const char* rfx_status_string(int status);
@@ -118,6 +119,83 @@ typedef struct {
     rfx_stream stream;
 } RfxKvLookupArgs;
 int rfx_kv_paged_lookup(const RfxKvLookupArgs* a);
+
+/* Page bookkeeping of a pool (no counterpart in the reference, whose caller owns the page tables).
+ * ref_counts [num_blocks] int32: requests that hold a page, 0 = free. Pages are handed out lowest first.
+ * The functions below only read and write tables and counts, on the device, and list the copies that
+ * follow from them (pairs of pages, -1 where there is none) for rfx_kv_copy_pages. num_blocks < 2^31.
+ *
+ * Fork: child i shares the whole pages of row parents[i] (their counts go up by one) and, where
+ * context_lens[parents[i]] ends inside a page, takes the lowest free page for itself (count 1), to which the
+ * filled positions have to be copied: src_pages[i], dst_pages[i], copy_rows[i] (else -1, -1, 0). Children
+ * take pages in order. child_table[i] gets the row, -1 behind it. A child for which no page is left has
+ * src_pages[i] >= 0 and dst_pages[i] = -1; it, and one whose parent is no row, gets a row of -1 and holds
+ * nothing. A table entry outside the pool is passed on as it is. Lengths are taken as at most
+ * max_blocks * block_size. */
+typedef struct {
+    const int64_t* block_table;  /* [batch, max_blocks], row stride bt_stride_b */
+    const int32_t* context_lens; /* [batch] */
+    const int32_t* parents;      /* [n_children] rows of block_table */
+    int32_t* ref_counts;         /* [num_blocks] */
+    int64_t* child_table;        /* [n_children, max_blocks] contiguous, fully written; not block_table itself */
+    int64_t* src_pages;          /* [n_children] */
+    int64_t* dst_pages;          /* [n_children] */
+    int32_t* copy_rows;          /* [n_children] positions to copy */
+    int64_t n_children, batch, max_blocks, bt_stride_b, num_blocks, block_size;
+    rfx_stream stream;
+} RfxKvForkArgs;
+int rfx_kv_fork(const RfxKvForkArgs* a);
+
+/* Free: every entry of the given rows becomes -1 and the count of its page goes down by one (never below
+ * zero). A row that is named twice, or freed before, gives its pages up once. */
+typedef struct {
+    int64_t* block_table;        /* [batch, max_blocks] */
+    const int32_t* rows;         /* [n_rows]; one outside the table is skipped */
+    int32_t* ref_counts;
+    int64_t n_rows, batch, max_blocks, bt_stride_b, num_blocks;
+    rfx_stream stream;
+} RfxKvFreeArgs;
+int rfx_kv_free(const RfxKvFreeArgs* a);
+
+/* Compact: with `live` pages in use, those at index live and behind move into the free pages below it, the
+ * last one into the first; table and counts follow. page_map[p] = the page's new index, -1 if it is free
+ * (so is a table entry that names a free page). The copies go to src_pages / dst_pages [num_blocks / 2 + 1]
+ * and their number to n_moves; no page is both source and destination. */
+typedef struct {
+    int64_t* block_table;        /* [batch, max_blocks], or NULL with batch 0 */
+    int32_t* ref_counts;
+    int64_t* page_map;           /* [num_blocks] */
+    int64_t* src_pages;
+    int64_t* dst_pages;
+    int32_t* n_moves;            /* device int */
+    int64_t batch, max_blocks, bt_stride_b, num_blocks;
+    void* workspace;             /* rfx_kv_compact_workspace_bytes(num_blocks) bytes */
+    size_t workspace_bytes;
+    rfx_stream stream;
+} RfxKvCompactArgs;
+size_t rfx_kv_compact_workspace_bytes(int64_t num_blocks);
+int rfx_kv_compact(const RfxKvCompactArgs* a);
+
+/* Copies page src_pages[i] onto page dst_pages[i] in the K and V caches of n_layers layers of one shape and
+ * stride pattern: its first copy_rows[i] positions (all of them without copy_rows; the others are left as
+ * they are). A pair with an index outside the pool, or onto itself, is skipped. Destinations must be
+ * distinct and none may be a source. int8 pools copy the scales too. */
+typedef struct {
+    void* const* k_caches;       /* host arrays of n_layers device pointers */
+    void* const* v_caches;
+    float* const* k_scales;      /* kv_int8 only */
+    float* const* v_scales;
+    const int64_t* src_pages;    /* [n_pairs] */
+    const int64_t* dst_pages;
+    const int32_t* copy_rows;    /* [n_pairs] or NULL */
+    const int32_t* n_moves;      /* device int or NULL: only the first *n_moves pairs */
+    int64_t n_layers, n_pairs, num_kv_heads, head_dim, num_blocks, block_size;
+    int64_t cache_stride_blk, cache_stride_h, cache_stride_pos;
+    int dtype;
+    int kv_int8;                 /* caches int8, scales [num_blocks, H_kv, block_size] */
+    rfx_stream stream;
+} RfxKvCopyArgs;
+int rfx_kv_copy_pages(const RfxKvCopyArgs* a);
 
 /* --------------------------------------------------------------------- rope ---- */
 

@@ -141,6 +141,10 @@ size_t rfx_args_size(int which) {
         case 10: return sizeof(RfxPeerHandle);
         case 11: return sizeof(RfxLinearNormArgs);
         case 12: return sizeof(RfxQkNormRopeArgs);
+        case 13: return sizeof(RfxKvForkArgs);
+        case 14: return sizeof(RfxKvFreeArgs);
+        case 15: return sizeof(RfxKvCompactArgs);
+        case 16: return sizeof(RfxKvCopyArgs);
         default: return 0;
     }
 }

@@ -58,6 +58,40 @@ class KvLookupArgs(C.Structure):
     ]
 
 
+class KvForkArgs(C.Structure):
+    _fields_ = [
+        ("block_table", vp), ("context_lens", vp), ("parents", vp), ("ref_counts", vp), ("child_table", vp),
+        ("src_pages", vp), ("dst_pages", vp), ("copy_rows", vp),
+        ("n_children", i64), ("batch", i64), ("max_blocks", i64), ("bt_stride_b", i64), ("num_blocks", i64),
+        ("block_size", i64), ("stream", vp),
+    ]
+
+
+class KvFreeArgs(C.Structure):
+    _fields_ = [
+        ("block_table", vp), ("rows", vp), ("ref_counts", vp),
+        ("n_rows", i64), ("batch", i64), ("max_blocks", i64), ("bt_stride_b", i64), ("num_blocks", i64), ("stream", vp),
+    ]
+
+
+class KvCompactArgs(C.Structure):
+    _fields_ = [
+        ("block_table", vp), ("ref_counts", vp), ("page_map", vp), ("src_pages", vp), ("dst_pages", vp), ("n_moves", vp),
+        ("batch", i64), ("max_blocks", i64), ("bt_stride_b", i64), ("num_blocks", i64),
+        ("workspace", vp), ("workspace_bytes", C.c_size_t), ("stream", vp),
+    ]
+
+
+class KvCopyArgs(C.Structure):
+    _fields_ = [
+        ("k_caches", C.POINTER(vp)), ("v_caches", C.POINTER(vp)), ("k_scales", C.POINTER(vp)), ("v_scales", C.POINTER(vp)),
+        ("src_pages", vp), ("dst_pages", vp), ("copy_rows", vp), ("n_moves", vp),
+        ("n_layers", i64), ("n_pairs", i64), ("num_kv_heads", i64), ("head_dim", i64), ("num_blocks", i64),
+        ("block_size", i64), ("cache_stride_blk", i64), ("cache_stride_h", i64), ("cache_stride_pos", i64),
+        ("dtype", C.c_int), ("kv_int8", C.c_int), ("stream", vp),
+    ]
+
+
 class RopeArgs(C.Structure):
     _fields_ = [
         ("x", vp), ("y", vp), ("cos", vp), ("sin", vp),
@@ -178,6 +212,11 @@ EXPORTS = {
     "rfx_kv_paged_append": (C.c_int, [C.POINTER(KvAppendArgs)]),
     "rfx_kv_paged_scatter": (C.c_int, [C.POINTER(KvAppendArgs)]),
     "rfx_kv_paged_lookup": (C.c_int, [C.POINTER(KvLookupArgs)]),
+    "rfx_kv_fork": (C.c_int, [C.POINTER(KvForkArgs)]),
+    "rfx_kv_free": (C.c_int, [C.POINTER(KvFreeArgs)]),
+    "rfx_kv_compact_workspace_bytes": (C.c_size_t, [i64]),
+    "rfx_kv_compact": (C.c_int, [C.POINTER(KvCompactArgs)]),
+    "rfx_kv_copy_pages": (C.c_int, [C.POINTER(KvCopyArgs)]),
     "rfx_rope_apply": (C.c_int, [C.POINTER(RopeArgs)]),
     "rfx_rope_build_tables": (C.c_int, [C.POINTER(RopeTableArgs)]),
     "rfx_rope_append": (C.c_int, [C.POINTER(RopeAppendArgs)]),
@@ -212,7 +251,7 @@ EXPORTS = {
 # Index of each mirror in rfx_args_size().
 ARG_STRUCTS = [KvAppendArgs, KvLookupArgs, RopeArgs, RopeTableArgs, RopeAppendArgs, SoftmaxArgs,
                AttentionArgs, PagedAttentionArgs, CombineArgs, HeadGatherArgs, PeerHandle, LinearNormArgs,
-               QkNormRopeArgs]
+               QkNormRopeArgs, KvForkArgs, KvFreeArgs, KvCompactArgs, KvCopyArgs]
 
 
 def library_path() -> Path:

@@ -8,10 +8,19 @@
 
 Pool layout ``[num_blocks, num_heads, block_size, head_dim]``, ``slot = page*block_size + pos``
 (``triton_kv_paged.py:9-15``). The caches are mutated in place.
+
+Page bookkeeping (additive; the reference leaves it to its caller), all of it on the device, with
+``ref_counts`` ``[num_blocks]`` int32 as its state (requests that hold a page, 0 = free):
+
+* ``kv_fork``       : children share their parent's whole pages, take a page for a part-filled last one.
+* ``kv_free``       : rows of the table give their pages up.
+* ``kv_compact``    : the live pages move to the front of the pool.
+* ``kv_copy_pages`` : the copies that fork and compact ask for (``PageMoves``), for all layers at once.
 """
 from __future__ import annotations
 
-from typing import Optional
+import ctypes as C
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -136,6 +145,208 @@ def kv_paged_scatter(
     _write_slots("rfx_kv_paged_scatter", "kv_paged_scatter", k_updates, v_updates, k_cache, v_cache, slot_mapping)
 
 
+class PageMoves(NamedTuple):
+    """Pages to copy: ``src[i]`` onto ``dst[i]`` (int64; a pair with -1 is none), the first ``rows[i]``
+    positions (int32; ``None``: all of them), for the first ``count[0]`` pairs (int32; ``None``: for all)."""
+
+    src: torch.Tensor
+    dst: torch.Tensor
+    rows: Optional[torch.Tensor] = None
+    count: Optional[torch.Tensor] = None
+
+
+def _check_table(name, block_table, ref_counts):
+    if block_table.dim() != 2 or block_table.dtype != torch.int64:
+        raise ValueError(f"{name}: block_table must be int64 [rows, max_blocks], "
+                         f"got {block_table.dtype} {tuple(block_table.shape)}")
+    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+        raise ValueError(f"{name}: the entries of a block_table row must be contiguous")
+    if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError(f"{name}: the rows of block_table overlap")
+    if ref_counts.dim() != 1 or ref_counts.dtype != torch.int32 or not ref_counts.is_contiguous():
+        raise ValueError(f"{name}: ref_counts must be contiguous int32 [num_blocks], "
+                         f"got {ref_counts.dtype} {tuple(ref_counts.shape)}")
+    if ref_counts.shape[0] == 0:
+        raise ValueError(f"{name}: ref_counts is empty")
+
+
+def _int32_vector(name, what, t, n=None):
+    if t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name}: {what} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise ValueError(f"{name}: {what} must hold whole numbers, got {t.dtype}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t.contiguous()
+
+
+def kv_fork(
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    parents: torch.Tensor,
+    ref_counts: torch.Tensor,
+    block_size: int,
+    *,
+    backend: Optional[str] = None,
+) -> Tuple[torch.Tensor, PageMoves]:
+    """Child ``i`` continues row ``parents[i]`` of ``block_table``: returns ``(child_table, moves)``.
+
+    A child shares its parent's whole pages (``ref_counts`` up by one each, in place). Where the parent's
+    ``context_lens`` ends inside a page the child takes the lowest free page for itself, and ``moves``
+    says which positions to copy there: give it to ``kv_copy_pages`` before the child's next token is
+    appended. ``child_table`` is ``[n, max_blocks]`` int64, -1 behind the child's pages. Children take free
+    pages in order; one for which none is left has ``moves.src >= 0`` and ``moves.dst < 0``, and it (and one
+    whose parent is no row) gets a row of -1 and holds nothing. A parent may have any number of children;
+    it keeps its own pages until ``kv_free``.
+    """
+    N.check_backend(backend)
+    name = "kv_fork"
+    dev = N.require_cuda(name, block_table, context_lens, parents, ref_counts)
+    _check_table(name, block_table, ref_counts)
+    if int(block_size) <= 0:
+        raise ValueError(f"{name}: block_size must be positive, got {block_size}")
+    batch, max_blocks = block_table.shape
+    context_lens = _int32_vector(name, "context_lens", context_lens, batch)
+    parents = _int32_vector(name, "parents", parents)
+    n = parents.shape[0]
+    child = torch.empty((n, max_blocks), dtype=torch.int64, device=dev)
+    pages = torch.empty((2, n), dtype=torch.int64, device=dev)
+    rows = torch.empty(n, dtype=torch.int32, device=dev)
+    src, dst = pages[0], pages[1]
+    a = N.KvForkArgs(
+        block_table=N.ptr(block_table), context_lens=N.ptr(context_lens), parents=N.ptr(parents),
+        ref_counts=N.ptr(ref_counts), child_table=N.ptr(child), src_pages=N.ptr(src), dst_pages=N.ptr(dst),
+        copy_rows=N.ptr(rows), n_children=n, batch=batch, max_blocks=max_blocks, bt_stride_b=block_table.stride(0),
+        num_blocks=ref_counts.shape[0], block_size=int(block_size), stream=N.stream_handle(dev),
+    )
+    N.call("rfx_kv_fork", a, dev)
+    return child, PageMoves(src, dst, rows)
+
+
+def kv_free(
+    block_table: torch.Tensor,
+    rows: torch.Tensor,
+    ref_counts: torch.Tensor,
+    *,
+    backend: Optional[str] = None,
+) -> None:
+    """The given rows of ``block_table`` give up every page they name: the entries become -1 and the
+    pages' ``ref_counts`` go down by one (in place). A row that is named twice or was freed before gives
+    its pages up once; a row outside the table is skipped."""
+    N.check_backend(backend)
+    name = "kv_free"
+    dev = N.require_cuda(name, block_table, rows, ref_counts)
+    _check_table(name, block_table, ref_counts)
+    rows = _int32_vector(name, "rows", rows)
+    a = N.KvFreeArgs(
+        block_table=N.ptr(block_table), rows=N.ptr(rows), ref_counts=N.ptr(ref_counts), n_rows=rows.shape[0],
+        batch=block_table.shape[0], max_blocks=block_table.shape[1], bt_stride_b=block_table.stride(0),
+        num_blocks=ref_counts.shape[0], stream=N.stream_handle(dev),
+    )
+    N.call("rfx_kv_free", a, dev)
+
+
+def kv_compact(
+    block_table: torch.Tensor,
+    ref_counts: torch.Tensor,
+    *,
+    backend: Optional[str] = None,
+) -> Tuple[torch.Tensor, PageMoves]:
+    """Moves the live pages to the front of the pool: returns ``(page_map, moves)``.
+
+    With ``live`` pages in use, those at index ``live`` and behind go into the free pages below it, the
+    last one into the first. ``block_table`` and ``ref_counts`` are rewritten in place; give ``moves`` to
+    ``kv_copy_pages`` before the pool is read again. ``page_map`` ``[num_blocks]`` int64 holds every page's
+    new index (-1: free), for tables other than this one; an entry of ``block_table`` that names a free
+    page becomes -1, one outside the pool is left as it is.
+    """
+    N.check_backend(backend)
+    name = "kv_compact"
+    dev = N.require_cuda(name, block_table, ref_counts)
+    _check_table(name, block_table, ref_counts)
+    num = ref_counts.shape[0]
+    page_map = torch.empty(num, dtype=torch.int64, device=dev)
+    pages = torch.empty((2, num // 2 + 1), dtype=torch.int64, device=dev)
+    need = int(N.lib().rfx_kv_compact_workspace_bytes(num))
+    # the number of moves stands in front of the scratch
+    words = torch.empty(64 + need // 4, dtype=torch.int32, device=dev)
+    src, dst, count = pages[0], pages[1], words[:1]
+    a = N.KvCompactArgs(
+        block_table=N.ptr(block_table), ref_counts=N.ptr(ref_counts), page_map=N.ptr(page_map), src_pages=N.ptr(src),
+        dst_pages=N.ptr(dst), n_moves=N.ptr(count), batch=block_table.shape[0], max_blocks=block_table.shape[1],
+        bt_stride_b=block_table.stride(0), num_blocks=num, workspace=words.data_ptr() + 256, workspace_bytes=need,
+        stream=N.stream_handle(dev),
+    )
+    N.call("rfx_kv_compact", a, dev)
+    return page_map, PageMoves(src, dst, None, count)
+
+
+def _layers(t):
+    return [t] if isinstance(t, torch.Tensor) else list(t)
+
+
+def kv_copy_pages(
+    k_cache: Union[torch.Tensor, Sequence[torch.Tensor]],
+    v_cache: Union[torch.Tensor, Sequence[torch.Tensor]],
+    moves: PageMoves,
+    *,
+    k_scales: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None,
+    v_scales: Union[None, torch.Tensor, Sequence[torch.Tensor]] = None,
+    backend: Optional[str] = None,
+) -> None:
+    """Copies pages inside the caches of one layer, or of all layers given as lists, in place.
+
+    ``moves`` comes from ``kv_fork`` or ``kv_compact`` or is a ``PageMoves`` of one's own. All layers share
+    one shape and stride pattern; int8 caches need their ``k_scales`` / ``v_scales`` ``[num_blocks, H_kv,
+    block_size]``, which move along. A pair with an index outside the pool is skipped; positions from
+    ``moves.rows[i]`` on are left as they are. Destinations must be distinct and none may be a source.
+    """
+    N.check_backend(backend)
+    name = "kv_copy_pages"
+    ks, vs = _layers(k_cache), _layers(v_cache)
+    if len(ks) != len(vs) or not ks:
+        raise ValueError(f"{name}: as many k as v caches are needed, at least one; got {len(ks)} and {len(vs)}")
+    src, dst, rows, count = moves
+    dev = N.require_cuda(name, *ks, *vs, src, dst, rows, count)
+    first = ks[0]
+    _check_pool(name, first, vs[0])
+    shape, strides, dtype = first.shape, first.stride(), first.dtype
+    for t in ks + vs:
+        if t.shape != shape or t.stride() != strides or t.dtype != dtype:
+            raise ValueError(f"{name}: the caches of all layers must share one shape, stride pattern and dtype")
+    if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.dim() != 1 or dst.shape != src.shape:
+        raise ValueError(f"{name}: moves.src and moves.dst must be int64 [n]")
+    n = src.shape[0]
+    src, dst = src.contiguous(), dst.contiguous()
+    if rows is not None:
+        rows = _int32_vector(name, "moves.rows", rows, n)
+    if count is not None and (count.dtype != torch.int32 or count.numel() != 1):
+        raise ValueError(f"{name}: moves.count must be one int32")
+    int8 = dtype == torch.int8
+    L = len(ks)
+    array = N.vp * L
+    a = N.KvCopyArgs(
+        k_caches=array(*[t.data_ptr() for t in ks]), v_caches=array(*[t.data_ptr() for t in vs]),
+        src_pages=N.ptr(src), dst_pages=N.ptr(dst), copy_rows=N.ptr(rows), n_moves=N.ptr(count),
+        n_layers=L, n_pairs=n, num_kv_heads=shape[1], head_dim=shape[3], num_blocks=shape[0], block_size=shape[2],
+        cache_stride_blk=strides[0], cache_stride_h=strides[1], cache_stride_pos=strides[2],
+        dtype=0 if int8 else N.dtype_code(first), kv_int8=int(int8), stream=N.stream_handle(dev),
+    )
+    if int8:
+        if k_scales is None or v_scales is None:
+            raise ValueError(f"{name}: an int8 pool needs k_scales and v_scales")
+        sk, sv = _layers(k_scales), _layers(v_scales)
+        N.require_cuda(name, first, *sk, *sv)
+        if len(sk) != L or len(sv) != L:
+            raise ValueError(f"{name}: every layer needs its scales")
+        for t in sk + sv:
+            if t.dtype != torch.float32 or t.shape != shape[:3] or not t.is_contiguous():
+                raise ValueError(f"{name}: scales must be contiguous float32 {list(shape[:3])}")
+        a.k_scales, a.v_scales = array(*[t.data_ptr() for t in sk]), array(*[t.data_ptr() for t in sv])
+    N.call("rfx_kv_copy_pages", a, dev)
+
+
+# The reference's surface; the page bookkeeping above is an addition, imported by name.
 __all__ = [
     "kv_paged_append",
     "kv_paged_lookup",
