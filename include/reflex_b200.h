@@ -62,7 +62,8 @@ int rfx_abi_version(void);
  * 2 RfxRopeArgs, 3 RfxRopeTableArgs, 4 RfxRopeAppendArgs, 5 RfxSoftmaxArgs,
  * 6 RfxAttentionArgs, 7 RfxPagedAttentionArgs, 8 RfxCombineArgs, 9 RfxHeadGatherArgs,
  * 10 RfxPeerHandle, 11 RfxLinearNormArgs, 12 RfxQkNormRopeArgs,
- * 13 RfxKvForkArgs, 14 RfxKvFreeArgs, 15 RfxKvCompactArgs, 16 RfxKvCopyArgs; 0 for anything else), so
+ * 13 RfxKvForkArgs, 14 RfxKvFreeArgs, 15 RfxKvCompactArgs, 16 RfxKvCopyArgs, 17 RfxSampleArgs;
+ * 0 for anything else), so
  * a foreign-function binding can verify its struct mirrors before the first call. */
 size_t rfx_args_size(int which);
 const char* rfx_status_string(int status);
@@ -328,6 +329,35 @@ typedef struct {
     rfx_stream stream;
 } RfxSoftmaxArgs;
 int rfx_online_softmax(const RfxSoftmaxArgs* a);
+
+/* One token per row of logits [batch, vocab], from a given uniform number (no counterpart in the reference):
+ *   l = the row's logits, NaN as -inf; z = (l - max) / temperature;
+ *   top_k: the k largest stay, of equal ones the lowest indexes (k <= 0 or k >= vocab: all);
+ *   w = exp(z) over those; top_p: in falling order (equal ones by index) a token stays while the mass
+ *   before it is below top_p * total, the first always (top_p >= 1 or NaN: all);
+ *   min_p: w >= min(min_p, 1) stays, the largest w being 1 (min_p <= 0 or NaN: all);
+ *   token = the lowest index at which the running sum of the staying w, in index order, exceeds
+ *   uniform * their sum (uniform >= 1: the last of weight, below 0 or NaN: the first).
+ * temperature <= 0 or NaN: the lowest index of the largest logit. A row with nothing but -inf (or NaN) gives
+ * -1; with +inf among its logits those share the mass. Every setting is a device array [batch], or with a
+ * NULL pointer one number for all rows. Weights are exp in 64 bits, summed as whole multiples of 2^-S of the
+ * largest, S = min(50, 62 - log2 vocab): the result depends on nothing but the arguments. vocab <= 2^24. */
+typedef struct {
+    const void* logits;          /* [batch, vocab], row stride below, last dim contiguous */
+    const float* uniform;        /* [batch], in [0, 1) */
+    const float* temperature;    /* [batch] or NULL: temperature_all */
+    const int32_t* top_k;        /* [batch] or NULL: top_k_all */
+    const float* top_p;          /* [batch] or NULL: top_p_all */
+    const float* min_p;          /* [batch] or NULL: min_p_all */
+    int64_t* tokens;             /* [batch] */
+    int64_t batch, vocab, row_stride;
+    float temperature_all;
+    int32_t top_k_all;
+    float top_p_all, min_p_all;
+    int dtype;
+    rfx_stream stream;
+} RfxSampleArgs;
+int rfx_sample_tokens(const RfxSampleArgs* a);
 
 /* ---------------------------------------------------------------- attention ---- */
 

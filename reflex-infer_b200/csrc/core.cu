@@ -145,6 +145,7 @@ size_t rfx_args_size(int which) {
         case 14: return sizeof(RfxKvFreeArgs);
         case 15: return sizeof(RfxKvCompactArgs);
         case 16: return sizeof(RfxKvCopyArgs);
+        case 17: return sizeof(RfxSampleArgs);
         default: return 0;
     }
 }

@@ -145,6 +145,15 @@ class SoftmaxArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", vp), ("uniform", vp), ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp), ("tokens", vp),
+        ("batch", i64), ("vocab", i64), ("row_stride", i64),
+        ("temperature_all", C.c_float), ("top_k_all", C.c_int32), ("top_p_all", C.c_float), ("min_p_all", C.c_float),
+        ("dtype", C.c_int), ("stream", vp),
+    ]
+
+
 class AttentionArgs(C.Structure):
     _fields_ = [
         ("q", vp), ("k", vp), ("v", vp), ("out", vp), ("attn_mask", vp),
@@ -223,6 +232,7 @@ EXPORTS = {
     "rfx_qk_norm_rope": (C.c_int, [C.POINTER(QkNormRopeArgs)]),
     "rfx_qk_norm_rope_append": (C.c_int, [C.POINTER(QkNormRopeArgs)]),
     "rfx_online_softmax": (C.c_int, [C.POINTER(SoftmaxArgs)]),
+    "rfx_sample_tokens": (C.c_int, [C.POINTER(SampleArgs)]),
     "rfx_fused_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionArgs)]),
     "rfx_fused_attention": (C.c_int, [C.POINTER(AttentionArgs)]),
     "rfx_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedAttentionArgs)]),
@@ -251,7 +261,7 @@ EXPORTS = {
 # Index of each mirror in rfx_args_size().
 ARG_STRUCTS = [KvAppendArgs, KvLookupArgs, RopeArgs, RopeTableArgs, RopeAppendArgs, SoftmaxArgs,
                AttentionArgs, PagedAttentionArgs, CombineArgs, HeadGatherArgs, PeerHandle, LinearNormArgs,
-               QkNormRopeArgs, KvForkArgs, KvFreeArgs, KvCompactArgs, KvCopyArgs]
+               QkNormRopeArgs, KvForkArgs, KvFreeArgs, KvCompactArgs, KvCopyArgs, SampleArgs]
 
 
 def library_path() -> Path:

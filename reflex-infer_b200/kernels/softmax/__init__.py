@@ -1,7 +1,11 @@
-"""Row softmax; same surface as the reference's ``kernels/softmax/__init__.py:15-35``."""
+"""Row softmax; same surface as the reference's ``kernels/softmax/__init__.py:15-35``.
+
+``sample_tokens`` (additive) draws a token from each row's softmax after temperature, top-k, top-p and
+min-p, with the random numbers given.
+"""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -38,4 +42,73 @@ def online_softmax(
     return y.reshape(x.shape)
 
 
+def _setting(name, what, value, B, dtype, low, high):
+    """``(tensor or None, number)`` of a sampling setting; only numbers are checked against their range."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (B,):
+            raise ValueError(f"{name}: {what} must be a number or [{B}], got {tuple(value.shape)}")
+        if value.dtype != dtype:
+            value = value.to(dtype)
+        return value.contiguous(), 0
+    if not low <= value <= high:
+        raise ValueError(f"{name}: {what} must be between {low} and {high}, got {value}")
+    return None, value
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniform: torch.Tensor,
+    *,
+    temperature: Union[float, torch.Tensor] = 1.0,
+    top_k: Union[int, torch.Tensor] = 0,
+    top_p: Union[float, torch.Tensor] = 1.0,
+    min_p: Union[float, torch.Tensor] = 0.0,
+    out: Optional[torch.Tensor] = None,
+    backend: Optional[str] = None,
+) -> torch.Tensor:
+    """One token per row of ``logits`` ``[B, vocab]`` from the numbers ``uniform`` ``[B]`` in [0, 1); returns
+    int64 ``[B]`` (``out`` if given).
+
+    Every setting is a number or a tensor ``[B]``. In this order: ``top_k`` keeps the k largest logits (0:
+    all); of their softmax at ``temperature`` ``top_p`` keeps the likeliest tokens while the mass before
+    them is below ``top_p``; ``min_p`` keeps those at least ``min_p`` times as likely as the likeliest. Equal
+    logits rank by index, the likeliest token always stays. The token is the lowest index at which the
+    running sum of the kept probabilities, in index order, exceeds ``uniform`` times their sum. Temperature 0
+    takes the largest logit. NaN counts as -inf; a row without a finite logit (or +inf) gives -1. Logits
+    may be strided by row; float64 settings and ``uniform`` are rounded to float32. The result depends on
+    the arguments alone, not on the batch, the launch or the order of threads; ``vocab`` is at most 2**24.
+    """
+    N.check_backend(backend)
+    name = "sample_tokens"
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"{name}: logits must be [B, vocab], got {tuple(logits.shape)}")
+    B, vocab = logits.shape
+    if uniform.shape != (B,):
+        raise ValueError(f"{name}: uniform must be [{B}], got {tuple(uniform.shape)}")
+    inf = float("inf")
+    temperature, temperature_all = _setting(name, "temperature", temperature, B, torch.float32, 0.0, inf)
+    top_k, top_k_all = _setting(name, "top_k", top_k, B, torch.int32, 0, inf)
+    top_p, top_p_all = _setting(name, "top_p", top_p, B, torch.float32, 0.0, 1.0)
+    min_p, min_p_all = _setting(name, "min_p", min_p, B, torch.float32, 0.0, 1.0)
+    dev = N.require_cuda(name, logits, uniform, temperature, top_k, top_p, min_p, out)
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    if uniform.dtype != torch.float32:
+        uniform = uniform.to(torch.float32)
+    uniform = uniform.contiguous()
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=dev)
+    elif out.shape != (B,) or out.dtype != torch.int64 or not out.is_contiguous():
+        raise ValueError(f"{name}: out must be contiguous int64 [{B}]")
+    a = N.SampleArgs(
+        logits=logits.data_ptr(), uniform=uniform.data_ptr(), temperature=N.ptr(temperature), top_k=N.ptr(top_k),
+        top_p=N.ptr(top_p), min_p=N.ptr(min_p), tokens=out.data_ptr(), batch=B, vocab=vocab, row_stride=logits.stride(0),
+        temperature_all=temperature_all, top_k_all=int(min(top_k_all, vocab)), top_p_all=top_p_all, min_p_all=min_p_all,
+        dtype=N.dtype_code(logits), stream=N.stream_handle(dev),
+    )
+    N.call("rfx_sample_tokens", a, dev)
+    return out
+
+
+# The reference's surface; sample_tokens is an addition, imported by name.
 __all__ = ["online_softmax"]

@@ -67,3 +67,13 @@ def test_page_refusals(native):
         assert lib.rfx_kv_copy_pages(C.byref(native.KvCopyArgs(**{**copy, **kw}))) == bad, kw
     for kw in (dict(n_pairs=0), dict(n_layers=0)):
         assert lib.rfx_kv_copy_pages(C.byref(native.KvCopyArgs(**{**copy, **kw}))) == native.RFX_SUCCESS
+
+
+def test_sample_refusals(native):
+    lib = native.lib()
+    good = dict(logits=256, uniform=256, tokens=256, batch=1, vocab=8, row_stride=8, temperature_all=1.0, top_p_all=1.0, dtype=1)
+    for kw in (dict(dtype=5), dict(batch=-1), dict(vocab=0), dict(vocab=-3), dict(vocab=(1 << 24) + 1), dict(logits=0),
+               dict(uniform=0), dict(tokens=0), dict(logits=257)):
+        assert lib.rfx_sample_tokens(C.byref(native.SampleArgs(**{**good, **kw}))) == native.RFX_INVALID_ARGUMENT, kw
+    assert lib.rfx_sample_tokens(None) == native.RFX_INVALID_ARGUMENT
+    assert lib.rfx_sample_tokens(C.byref(native.SampleArgs(**{**good, "batch": 0}))) == native.RFX_SUCCESS
