@@ -10,17 +10,23 @@
 // S = min(50, 62 - log2 V), and added up as a 64-bit integer. Such sums are exact in any order; what a weight
 // loses (2^-S-1 of the largest, 2^-46 at 131072 tokens) is far below the distance of two borders.
 //
-// A cluster of up to 8 CTAs takes a row, each a slice of it, which stays in shared memory: the logits are read
-// from HBM once (algorithmic bytes: V*e a row). Two ways to the answer:
-//   list     (top-k up to 512 a CTA) every thread's largest logit is known from the load; the ceil(k/C)-th largest of
-//            those, lowest over the CTAs, bounds the k-th largest logit from below. What lies above it (about 1.4 k
-//            logits) is sorted by one CTA, which then has the whole kept set in hand.
-//   general  a histogram over max - l (counts for top-k, masses for top-p) names the bin with the border,
-//            the logits of that bin are sorted, and a pass in index order adds up what is kept. Without
-//            top-k and top-p only that pass is left.
+// A cluster of up to 8 CTAs takes a row, each a slice of it (one CTA a row in large batches). Two ways to the
+// answer, by the row's settings:
+//   list     (top-k up to 512) The logits stream through registers once. Every thread keeps the largest of two groups
+//            of its own; the k-th largest of the CTA's 1024 group maxima bounds the k-th largest logit from below, and
+//            what reaches the bound, renewed whenever the logits seen have doubled, goes to a list in shared
+//            memory. About 1.3 k logits are left in the end; one CTA ranks them, and has the kept set in hand.
+//   general  The slice stays in shared memory (or is read again from L2). A histogram over max - l (counts for top-k,
+//            masses for top-p) names the bin with the border, the logits of that bin are ranked, and a pass in index
+//            order adds up what is kept. Without top-k and top-p only that pass is left.
 // A list that overflows (thousands of equal logits) is replaced by a search over the bits of the border's
 // key and index: slower, and right for every input.
+//
+// Algorithmic bytes: V*e a row, read once. List rows are bound by HBM in large batches and by the dozen barriers and
+// three cluster barriers of a row in small ones; general rows by the 64-bit exponentials, one a logit.
 #include <cooperative_groups.h>
+
+#include <utility>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -32,11 +38,16 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kCap = 2048;   // logits that one CTA sorts
+constexpr int kCap = 2048;     // logits that one CTA ranks
+constexpr int kPairs = 512;    // up to here by comparing all pairs, behind by sorting
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-constexpr size_t kStageTwo = 78 * 1024;   // slice that lets two CTAs share an SM
-constexpr size_t kStageMax = 188 * 1024;  // largest slice kept in shared memory
+constexpr int kGroups = 2 * kThreads;     // groups whose maxima bound the k-th largest logit
+constexpr int kListK = kGroups / 2;       // with k near kGroups the bound sinks to the smallest of the maxima
+constexpr int kBatch = 4;                 // 16-byte chunks a thread has under way
+constexpr size_t kStageTwo = 72 * 1024;   // slice that lets two CTAs share an SM
+constexpr size_t kStageMax = 180 * 1024;  // largest slice kept in shared memory
+constexpr float kLowest = -3.402823466e38f;
 
 struct SampleParams {
     const void* logits;
@@ -48,40 +59,80 @@ struct SampleParams {
     int32_t top_k0;
     int vocab, slice;  // slice: logits per CTA, a multiple of 8
     int shift;         // S: weights are multiples of 2^-S
+    int staged;        // general rows keep their slice in shared memory
 };
 
-struct Shared {
+struct __align__(16) Entry { u64 key, mass; };  // key: the logit's ordered bits, then ~index
+
+struct __align__(16) Shared {
     u64 list[kCap];
     union {
         struct { uint32_t lo[kBins], hi[kBins]; } hist;
-        u64 weight[kCap];  // of the sorted list
+        u64 weight[kCap];       // of the sorted list
+        Entry pair[kPairs];     // of the list where all pairs are compared
+        uint32_t group[kGroups];
     };
     u64 part[kWarps];
-    u64 slot[2];
-    u64 found[2];  // what rank 0 tells the others
-    int n;         // entries that want to be in `list`
+    u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
+    u64 found[3];              // what rank 0 tells everyone
+    uint32_t picked[3];        // of select(): the bound, the largest key, n before it
+    int n;                     // entries that want to be in `list`
 };
 
 __device__ __forceinline__ uint32_t key_of(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.f);  // -0 and +0 are one value
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+// The smallest finite value that a key, or any bits below those of -inf, lets through: never -inf or NaN.
+__device__ __forceinline__ float bound_of(uint32_t k) { return k <= 0x00800000u ? kLowest : value_of(k); }
 
 template <typename T> struct Chunk {  // 16 bytes of logits
     static constexpr int N = 16 / sizeof(T);
     union { uint4 raw; T v[N]; };
     __device__ Chunk() {}
     __device__ __forceinline__ float at(int e) const {
-        const float f = Num<T>::to_f(v[e]) + 0.f;  // -0 and +0 are one value
-        return f == f ? f : -INFINITY;             // NaN counts as masked
+        const float f = Num<T>::to_f(v[e]) + 0.f;
+        return f == f ? f : -INFINITY;  // NaN counts as masked
+    }
+    __device__ __forceinline__ float raw_at(int e) const { return Num<T>::to_f(v[e]); }
+    // The largest that is no NaN; -inf if all are.
+    __device__ __forceinline__ float most() const {
+        if constexpr (sizeof(T) == 4) {
+            return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), -INFINITY);
+        } else {
+            using W = typename Pair16<T>::P;
+            const W* w = reinterpret_cast<const W*>(v);
+            const float2 f = Pair16<T>::widen(__hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3])));
+            return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+        }
     }
 };
 
+// Bitonic sort of list[0, n), falling. A stage whose pairs stay inside a warp's 64 entries needs no block barrier.
+__device__ __noinline__ void sort_list(u64* list, int n) {
+    int n2 = 64;
+    while (n2 < n) n2 *= 2;
+    __syncthreads();
+    for (int i = n + threadIdx.x; i < n2; i += kThreads) list[i] = 0;
+    __syncthreads();
+    for (int size = 2; size <= n2; size *= 2) {
+        for (int stride = size / 2; stride > 0; stride /= 2) {
+            for (int t = threadIdx.x; t < n2 / 2; t += kThreads) {
+                const int i = 2 * t - (t & (stride - 1));
+                const u64 a = list[i], b = list[i + stride];
+                if ((a < b) == ((i & size) == 0)) { list[i] = b; list[i + stride] = a; }
+            }
+            if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads(); else __syncwarp();
+        }
+    }
+    __syncthreads();
+}
+
 // One CTA's view of its row.
-template <typename T, bool STAGED> struct Row {
+template <typename T> struct Row {
     static constexpr int N = Chunk<T>::N;
     const T* row;    // the row's logits
     T* stage;        // the slice in shared memory, at the 16-byte phase it has in global memory
@@ -89,11 +140,13 @@ template <typename T, bool STAGED> struct Row {
     int base, nvec;  // 16-byte chunks from index `base` (lo rounded down to the boundary)
     Shared& s;
     int rank, ranks, parity;
-    float top;            // the row's largest logit
-    double scale;         // log-weight per unit: 1 / T
-    double unit;          // 2^S
-    float bins;           // histogram bins per unit
     int vocab;
+    bool staged;
+    float top;            // the row's largest logit
+    double scale;         // log2-weight per unit: log2(e) / T
+    double unit;          // 2^S
+    int shift;            // S
+    float bins;           // histogram bins per unit
     uint32_t cut_key;     // kept: key > cut_key, or key == cut_key and index <= cut_index
     int cut_index;
 
@@ -109,7 +162,7 @@ template <typename T, bool STAGED> struct Row {
         return c;
     }
     __device__ __forceinline__ Chunk<T> load(int j) const {
-        if (!STAGED) return load_global(j);
+        if (!staged) return load_global(j);
         Chunk<T> c;
         c.raw = reinterpret_cast<const uint4*>(stage)[j];
         return c;
@@ -122,10 +175,35 @@ template <typename T, bool STAGED> struct Row {
             for (int e = 0; e < N; ++e) f(c.at(e), base + j * N + e);
         }
     }
+    // exp((v - top) / T) * 2^S, 0 where that is below a quarter. 2^t = 2^n * 2^f with n whole and |f| <= 1/2, and
+    // 2^f = sum (f ln 2)^k / k! to k = 12: the first term left out is below 2e-16 of the sum.
     __device__ __forceinline__ double weight(float v) const {
-        return v == top ? 1.0 : exp(((double)v - (double)top) * scale);
+        const double t = v == top ? 0.0 : ((double)v - (double)top) * scale;
+        if (!(t >= -(double)(shift + 2))) return 0.0;
+        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+        const double n = t + kMagic;
+        const double f = t - (n - kMagic);
+        double w = 2.5678435993488196e-11;   // ln2^12 / 12!
+        w = fma(w, f, 4.44553827187081e-10);
+        w = fma(w, f, 7.054911620801121e-09);
+        w = fma(w, f, 1.0178086009239696e-07);
+        w = fma(w, f, 1.3215486790144305e-06);
+        w = fma(w, f, 1.5252733804059838e-05);
+        w = fma(w, f, 0.00015403530393381606);
+        w = fma(w, f, 0.0013333558146428441);
+        w = fma(w, f, 0.009618129107628477);
+        w = fma(w, f, 0.055504108664821576);
+        w = fma(w, f, 0.2402265069591007);
+        w = fma(w, f, 0.6931471805599453);
+        w = fma(w, f, 1.0);
+        const int e = __double2loint(n) + shift;
+        return __hiloint2double(__double2hiint(w) + (e << 20), __double2loint(w));
     }
-    __device__ __forceinline__ u64 fixed(double w) const { return (u64)__double2ll_rn(w * unit); }
+    // To a whole number: below 2^52 the sum with 2^52 holds it in its low bits.
+    __device__ __forceinline__ u64 fixed(double w) const {
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ u64 mass(uint32_t key) const { return fixed(weight(value_of(key))); }
     __device__ __forceinline__ bool kept(float v, int i) const {
         const uint32_t k = key_of(v);
         return v > -INFINITY && (k > cut_key || (k == cut_key && i <= cut_index));
@@ -136,9 +214,13 @@ template <typename T, bool STAGED> struct Row {
         return x < (float)kBins ? (int)x : kBins;
     }
 
-    __device__ __forceinline__ u64 block_sum(u64 v) {
+    __device__ __forceinline__ static u64 warp_total(u64 v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    __device__ __forceinline__ u64 block_sum(u64 v) {
+        v = warp_total(v);
         __syncthreads();
         if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = v;
         __syncthreads();
@@ -168,81 +250,61 @@ template <typename T, bool STAGED> struct Row {
         }
         return before + x - v;
     }
-    // Every CTA's word, seen by all: word(r) after the call. Two slots in turn: a CTA writes a slot again only
-    // after the next exchange, which the readers of this one have reached by then.
-    __device__ __forceinline__ u64* exchange(u64 mine) {
+    // Every CTA's word: CTA r's in lane r, 0 behind the last. A CTA writes its word into the others' shared memory, so
+    // that after the barrier everyone reads its own. Two sets of slots in turn: one is written again only after the
+    // next exchange, which the readers of this one have reached by then. Thread 0's word counts; every CTA of the
+    // cluster must have started (see the kernel).
+    __device__ __forceinline__ u64 exchange(u64 mine) {
         parity ^= 1;
-        if (threadIdx.x == 0) s.slot[parity] = mine;
+        const int lane = threadIdx.x & 31;
+        if (threadIdx.x < 32) {
+            mine = __shfl_sync(0xffffffffu, mine, 0);
+            if (lane < ranks) *cg::this_cluster().map_shared_rank(&s.slot[parity][rank], lane) = mine;
+        }
         cg::this_cluster().sync();
-        return &s.slot[parity];
+        return lane < ranks ? s.slot[parity][lane] : 0;
     }
-    __device__ __forceinline__ u64 word(u64* slot, int r) const { return *cg::this_cluster().map_shared_rank(slot, r); }
-    __device__ __forceinline__ u64 cluster_sum(u64 v) {
-        u64* slot = exchange(block_sum(v));
-        u64 t = 0;
-        for (int r = 0; r < ranks; ++r) t += word(slot, r);
-        return t;
-    }
-    // Two words from rank 0 to everyone.
-    __device__ __forceinline__ void tell(u64& a, u64& b) {
-        if (rank == 0 && threadIdx.x == 0) { s.found[0] = a; s.found[1] = b; }
+    __device__ __forceinline__ u64 cluster_sum(u64 v) { return warp_total(exchange(block_sum(v))); }
+    // Three words of rank 0's thread 0 to everyone. Between two calls lies an exchange.
+    __device__ __forceinline__ void tell(u64& a, u64& b, u64& c) {
+        if (rank == 0 && threadIdx.x == 0) {
+            for (int r = 0; r < ranks; ++r) {
+                u64* f = cg::this_cluster().map_shared_rank(s.found, r);
+                f[0] = a; f[1] = b; f[2] = c;
+            }
+        }
         cg::this_cluster().sync();
-        const u64* f = cg::this_cluster().map_shared_rank(s.found, 0);
-        a = f[0];
-        b = f[1];
-        cg::this_cluster().sync();
+        a = s.found[0];
+        b = s.found[1];
+        c = s.found[2];
     }
 
-    // Puts the logits that `want` takes into rank 0's list; returns their number (the list holds them all
-    // only up to kCap).
-    template <typename F> __device__ __forceinline__ int gather(F want) {
+    __device__ __forceinline__ void put(float v, int i) {
+        const int at = atomicAdd(&s.n, 1);
+        if (at < kCap) s.list[at] = (u64)key_of(v) << 32 | (0xffffffffu - (uint32_t)i);
+    }
+    // Rank 0 collects the CTAs' lists; returns the entries of all of them (the list holds them only up to kCap).
+    __device__ __forceinline__ int collect() {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         __syncthreads();
-        if (threadIdx.x == 0) s.n = 0;
-        __syncthreads();
-        each([&](float v, int i) {
-            if (!want(v, i)) return;
-            const int at = atomicAdd(&s.n, 1);
-            if (at < kCap) s.list[at] = (u64)key_of(v) << 32 | (0xffffffffu - (uint32_t)i);
-        });
-        __syncthreads();
-        u64* slot = exchange((u64)(unsigned)s.n);
-        int total = 0;
-        for (int r = 0; r < ranks; ++r) total += (int)word(slot, r);
-        if (rank == 0 && total <= kCap) {
-            int at = s.n;
-            for (int r = 1; r < ranks; ++r) {
-                const int n = (int)word(slot, r);
+        const int n = (int)exchange((u64)(unsigned)s.n);
+        const int total = (int)warp_total((u64)n);
+        if (rank == 0 && total <= kCap && ranks > 1) {
+            // a CTA's list is pulled by the kWarps / kMaxCluster warps of its number
+            const int r = warp % kMaxCluster;
+            const int at = __reduce_add_sync(0xffffffffu, lane < r ? n : 0);
+            const int mine = __shfl_sync(0xffffffffu, n, r);
+            if (r > 0 && r < ranks) {
                 const u64* from = cg::this_cluster().map_shared_rank(s.list, r);
-                for (int x = threadIdx.x; x < n; x += kThreads) s.list[at + x] = from[x];
-                at += n;
+                for (int x = warp / kMaxCluster * 32 + lane; x < mine; x += kWarps / kMaxCluster * 32) s.list[at + x] = from[x];
             }
-            __syncthreads();
         }
+        __syncthreads();
         return total;
     }
-    // Bitonic sort of list[0, n), falling. A stage whose pairs stay inside a warp's 64 entries needs no block barrier.
-    __device__ void sort(int n) {
-        int n2 = 64;
-        while (n2 < n) n2 *= 2;
-        __syncthreads();
-        for (int i = n + threadIdx.x; i < n2; i += kThreads) s.list[i] = 0;
-        __syncthreads();
-        for (int size = 2; size <= n2; size *= 2) {
-            for (int stride = size / 2; stride > 0; stride /= 2) {
-                for (int t = threadIdx.x; t < n2 / 2; t += kThreads) {
-                    const int i = 2 * t - (t & (stride - 1));
-                    const u64 a = s.list[i], b = s.list[i + stride];
-                    if ((a < b) == ((i & size) == 0)) { s.list[i] = b; s.list[i + stride] = a; }
-                }
-                if (stride > 32 || (stride == 1 && size >= 64)) __syncthreads(); else __syncwarp();
-            }
-        }
-        __syncthreads();
-    }
-
     // The border of a sum over the kept logits in falling order: count (top-k) or mass (top-p) up to and
     // including the border first reaches the target. Moves the cut there.
-    template <bool MASS> __device__ void cut(int k, float p) {
+    template <bool MASS> __device__ __forceinline__ void cut(int k, float p) {
         for (int b = threadIdx.x; b < kBins; b += kThreads) s.hist.lo[b] = s.hist.hi[b] = 0;
         __syncthreads();
         each([&](float v, int i) {
@@ -258,67 +320,76 @@ template <typename T, bool STAGED> struct Row {
                 atomicAdd(&s.hist.lo[b], 1u);
             }
         });
+        if (threadIdx.x == 0) s.found[0] = ~0ull;
         cg::this_cluster().sync();
-        u64 at = ~0ull, above = 0, target = (u64)k;
+        u64 at = 0, above = 0, target = (u64)k;
         if (rank == 0) {
-            constexpr int PER = kBins / kThreads;
-            u64 m[PER], sum = 0, total;
+            static_assert(kBins == 4 * kThreads, "a thread's bins are one 16-byte vector");
+            u64 m[4] = {0, 0, 0, 0}, total;
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int b = threadIdx.x * PER + j;
-                m[j] = 0;
-                for (int r = 0; r < ranks; ++r) {
-                    m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
-                    m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
+            for (int r = 0; r < kMaxCluster; ++r) {  // all CTAs' bins under way together
+                if (r >= ranks) continue;
+                const uint4 l = reinterpret_cast<const uint4*>(cg::this_cluster().map_shared_rank(s.hist.lo, r))[threadIdx.x];
+                m[0] += l.x; m[1] += l.y; m[2] += l.z; m[3] += l.w;
+                if (MASS) {
+                    const uint4 h = reinterpret_cast<const uint4*>(cg::this_cluster().map_shared_rank(s.hist.hi, r))[threadIdx.x];
+                    m[0] += (u64)h.x << 32; m[1] += (u64)h.y << 32; m[2] += (u64)h.z << 32; m[3] += (u64)h.w << 32;
                 }
-                sum += m[j];
             }
-            u64 before = block_scan(sum, total);
+            u64 before = block_scan(m[0] + m[1] + m[2] + m[3], total);
             if (MASS) target = target_of(p, total);
-            if (threadIdx.x == 0) { s.found[0] = ~0ull; s.found[1] = 0; }
-            __syncthreads();
+            if (MASS || total > target) {  // else the border lies behind the last logit that weighs anything
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                if (before < target && before + m[j] >= target && total > target - (MASS ? 1 : 0)) {
-                    s.found[0] = (u64)(threadIdx.x * PER + j);
-                    s.found[1] = before;
-                    s.slot[parity ^ 1] = target;  // free until the next exchange
+                for (int j = 0; j < 4; ++j) {
+                    if (before < target && before + m[j] >= target) {
+                        s.found[0] = (u64)(threadIdx.x * 4 + j);
+                        s.found[1] = before;
+                    }
+                    before += m[j];
                 }
-                before += m[j];
             }
             __syncthreads();
+            at = s.found[0];
+            above = s.found[1];
         }
-        cg::this_cluster().sync();
-        at = *cg::this_cluster().map_shared_rank(&s.found[0], 0);
-        above = *cg::this_cluster().map_shared_rank(&s.found[1], 0);
-        target = *cg::this_cluster().map_shared_rank(&s.slot[parity ^ 1], 0);
-        cg::this_cluster().sync();
-        if (at == ~0ull) return;  // the border lies behind the last logit that weighs anything
+        tell(at, above, target);
+        if (at == ~0ull) return;
         const int bin = (int)at;
-        const int n = gather([&](float v, int i) { return kept(v, i) && bin_of(v) == bin; });
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        each([&](float v, int i) {
+            if (bin_of(v) == bin && kept(v, i)) put(v, i);
+        });
+        const int n = collect();
         if (n <= kCap) {
-            u64 key = 0, index = 0;
+            u64 key = 0, unused = 0, unused2 = 0;
             if (rank == 0) {
-                sort(n);
-                constexpr int PER = kCap / kThreads;
-                u64 m[PER], sum = 0, total;
+                if (n <= kPairs) {
+                    rank_pairs<MASS>(n, [&](u64 e, int, u64 before, u64 m) {
+                        before += above;
+                        if (before < target && before + m >= target) s.found[0] = e;
+                    });
+                } else {
+                    sort_list(s.list, n);
+                    constexpr int PER = kCap / kThreads;
+                    u64 m[PER], sum = 0, total;
 #pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const int i = threadIdx.x * PER + j;
-                    m[j] = i < n ? (MASS ? fixed(weight(value_of((uint32_t)(s.list[i] >> 32)))) : 1) : 0;
-                    sum += m[j];
-                }
-                u64 before = above + block_scan(sum, total);
+                    for (int j = 0; j < PER; ++j) {
+                        const int i = threadIdx.x * PER + j;
+                        m[j] = i < n ? (MASS ? mass((uint32_t)(s.list[i] >> 32)) : 1) : 0;
+                        sum += m[j];
+                    }
+                    u64 before = above + block_scan(sum, total);
 #pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    if (before < target && before + m[j] >= target) s.found[0] = s.list[threadIdx.x * PER + j];
-                    before += m[j];
+                    for (int j = 0; j < PER; ++j) {
+                        if (before < target && before + m[j] >= target) s.found[0] = s.list[threadIdx.x * PER + j];
+                        before += m[j];
+                    }
                 }
                 __syncthreads();
                 key = s.found[0];
-                __syncthreads();
             }
-            tell(key, index);
+            tell(key, unused, unused2);
             cut_key = (uint32_t)(key >> 32);
             cut_index = (int)(0xffffffffu - (uint32_t)key);
             return;
@@ -327,7 +398,7 @@ template <typename T, bool STAGED> struct Row {
         auto sum_from = [&](uint32_t from) {  // over the bin's logits with keys >= from
             u64 t = 0;
             each([&](float v, int i) {
-                if (kept(v, i) && bin_of(v) == bin && key_of(v) >= from) t += MASS ? fixed(weight(v)) : 1;
+                if (bin_of(v) == bin && key_of(v) >= from && kept(v, i)) t += MASS ? fixed(weight(v)) : 1;
             });
             return above + cluster_sum(t);
         };
@@ -335,23 +406,22 @@ template <typename T, bool STAGED> struct Row {
         for (int bit = 31; bit >= 0; --bit)
             if (sum_from(key | 1u << bit) >= target) key |= 1u << bit;
         const u64 over = key == 0xffffffffu ? above : sum_from(key + 1);
-        const u64 each_w = MASS ? fixed(weight(value_of(key))) : 1;
-        const u64 ties = (target - over + each_w - 1) / each_w;  // equal logits that stay
-        const uint32_t old_key = cut_key;
-        const int old_index = cut_index;
-        int index = -1;  // largest index with fewer than `ties` equal ones up to it, then the next
+        const u64 each_one = MASS ? mass(key) : 1;
+        const u64 ties = (target - over + each_one - 1) / each_one;  // equal logits that stay
+        int index = -1;  // largest index with fewer than `ties` equal ones up to it
         for (int bit = 24; bit >= 0; --bit) {
             const int to = index + (1 << bit);
             if (to >= vocab) continue;
             u64 t = 0;
             each([&](float v, int i) {
-                if (v > -INFINITY && key_of(v) == key && (key > old_key || i <= old_index) && i <= to) ++t;
+                if (i <= to && key_of(v) == key && kept(v, i)) ++t;
             });
             if (cluster_sum(t) < ties) index = to;
         }
         cut_key = key;
         cut_index = index + 1;
     }
+
     // Sums below p of the total; the first logit always stays.
     __device__ __forceinline__ u64 target_of(float p, u64 total) const {
         const double t = ceil((double)p * (double)total);
@@ -362,12 +432,14 @@ template <typename T, bool STAGED> struct Row {
         const u64 x = t > 0.0 ? (u64)t : 0;  // a NaN draws the first
         return x < total ? x : total - 1;
     }
+    // Smallest weight that stays, in units of 2^-S.
+    __device__ __forceinline__ double least_of(float min_p) const { return min_p > 0.f ? fmin((double)min_p, 1.0) * unit : 0.0; }
 
     // The draw over everything kept: sums per warp over neighbouring logits, then one warp looks closer.
-    __device__ void draw(float u, float min_p, int64_t* token) {
+    __device__ __forceinline__ void draw(float u, float min_p, int64_t* token) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const int per = (nvec + kWarps - 1) / kWarps, from = warp * per, to = min(nvec, from + per);
-        const double least = (min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0);
+        const double least = least_of(min_p);
         auto of = [&](float v, int i) -> u64 {
             if (!kept(v, i)) return 0;
             const double w = weight(v);
@@ -379,9 +451,7 @@ template <typename T, bool STAGED> struct Row {
 #pragma unroll
             for (int e = 0; e < N; ++e) sum += of(c.at(e), base + j * N + e);
         }
-        u64 all = sum;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        const u64 all = warp_total(sum);
         __syncthreads();
         if (lane == 0) s.part[warp] = all;
         __syncthreads();
@@ -390,13 +460,9 @@ template <typename T, bool STAGED> struct Row {
             if (w < warp) before += s.part[w];
             mine += s.part[w];
         }
-        u64* slot = exchange(mine);
-        u64 total = 0;
-        for (int r = 0; r < ranks; ++r) {
-            const u64 x = word(slot, r);
-            if (r < rank) before += x;
-            total += x;
-        }
+        const u64 each_cta = exchange(mine);
+        const u64 total = warp_total(each_cta);
+        before += warp_total(lane < rank ? each_cta : 0);
         const u64 target = drawn(u, total);
         if (target < before || target >= before + all) return;  // whole warps
         for (int j0 = from; j0 < to; j0 += 32) {
@@ -429,12 +495,58 @@ template <typename T, bool STAGED> struct Row {
         }
     }
 
+    // f(entry, its place, the sum before it, its own mass or 1) for list[0, n), n <= kPairs, all in falling order,
+    // without sorting: a thread compares its entry with every other.
+    template <bool MASS, typename F> __device__ __forceinline__ void rank_pairs(int n, F f) {
+        const int i = threadIdx.x;
+        Entry mine = {0, 0};
+        if (i < n) {
+            mine.key = s.list[i];
+            mine.mass = MASS ? mass((uint32_t)(mine.key >> 32)) : 1;
+            s.pair[i] = mine;
+        }
+        __syncthreads();
+        if (i >= n) return;
+        int place = 0;
+        u64 before = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const Entry o = s.pair[j];
+            if (o.key > mine.key) { ++place; before += o.mass; }
+        }
+        f(mine.key, place, before, mine.mass);
+    }
+
     // rank 0, with the largest logits in list[0, n): everything that is left to do
-    __device__ void finish_list(int n, int k, float p, float min_p, float u, int64_t* token) {
-        sort(n);
+    __device__ __forceinline__ void finish_list(int n, int k, float p, float min_p, float u, int64_t* token) {
+        const double least = least_of(min_p);
+        if (n <= kPairs) {
+            u64 key = 0, before = 0, m = 0;
+            bool in = false;
+            rank_pairs<true>(n, [&](u64 e, int place, u64 b, u64 w) { key = e; before = b; m = w; in = place < k; });
+            const u64 total = block_sum(in ? m : 0);  // (its barrier also ends the reading of s.pair)
+            if (p < 1.f) in = in && before < target_of(p, total);
+            in = in && weight(value_of((uint32_t)(key >> 32))) >= least;
+            if (!in) m = 0;
+            const u64 sum = block_sum(m);
+            if (threadIdx.x < n) s.pair[threadIdx.x] = Entry{key << 32, m};  // falling in ~index: rising in index
+            __syncthreads();
+            if (!in) return;
+            u64 at = 0;
+            key <<= 32;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+                const Entry o = s.pair[j];
+                if (o.key > key) at += o.mass;
+            }
+            const u64 x = drawn(u, sum);
+            if (x >= at && x < at + m) *token = (int64_t)(0xffffffffu - (uint32_t)(key >> 32));
+            return;
+        }
+        sort_list(s.list, n);
         if (k < n) n = k;
         constexpr int PER = kCap / kThreads;
-        u64 m[PER], sum = 0, total, unused;
+        u64 m[PER], sum = 0, total;
         double w[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -445,7 +557,6 @@ template <typename T, bool STAGED> struct Row {
         }
         u64 before = block_scan(sum, total);
         const u64 target = p < 1.f ? target_of(p, total) : ~0ull;
-        const double least = (min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0);
         int stay = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -468,7 +579,7 @@ template <typename T, bool STAGED> struct Row {
             const int i = threadIdx.x * PER + j;
             if (i < kept_n) { s.list[i] = e[j]; s.weight[i] = m[j]; }
         }
-        sort(kept_n);
+        sort_list(s.list, kept_n);
         sum = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -477,32 +588,187 @@ template <typename T, bool STAGED> struct Row {
             m[j] = i < kept_n ? s.weight[(uint32_t)e[j]] : 0;
             sum += m[j];
         }
-        u64 at = block_scan(sum, unused);
-        const u64 x = drawn(u, unused);
+        u64 at = block_scan(sum, total);
+        const u64 x = drawn(u, total);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             if (x >= at && x < at + m[j]) *token = (int64_t)(0xffffffffu - (uint32_t)(e[j] >> 32));
             at += m[j];
         }
     }
+
+    // A key that at least `count` of the CTA's group maxima reach (0 if there are fewer groups with logits), within 2^-10 of the
+    // spread of the maxima's bits below the count-th; and their largest key. One warp searches, bit by bit.
+    __device__ __forceinline__ uint32_t select(const float (&most)[2], int count, uint32_t& largest) {
+        s.group[threadIdx.x] = key_of(most[0]);
+        s.group[kThreads + threadIdx.x] = key_of(most[1]);
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            uint32_t k[kGroups / 32], high = 0, low = 0xffffffffu;
+#pragma unroll
+            for (int x = 0; x < kGroups / 128; ++x) {
+                const uint4 v = reinterpret_cast<const uint4*>(s.group)[x * 32 + threadIdx.x];
+                k[4 * x] = v.x; k[4 * x + 1] = v.y; k[4 * x + 2] = v.z; k[4 * x + 3] = v.w;
+            }
+#pragma unroll
+            for (int x = 0; x < kGroups / 32; ++x) { high = max(high, k[x]); low = min(low, k[x]); }
+            high = __reduce_max_sync(0xffffffffu, high);
+            low = __reduce_min_sync(0xffffffffu, low);
+            uint32_t bound = high;
+            if (high != low) {
+                const int first = 31 - __clz(high ^ low);
+                bound = first == 31 ? 0 : high >> (first + 1) << (first + 1);
+                for (int bit = first; bit >= max(0, first - 9); --bit) {
+                    const uint32_t next = bound | 1u << bit;
+                    int c = 0;
+#pragma unroll
+                    for (int x = 0; x < kGroups / 32; ++x) c += k[x] >= next;
+                    if (__reduce_add_sync(0xffffffffu, c) >= count) bound = next;
+                }
+            }
+            if (threadIdx.x == 0) { s.picked[0] = bound; s.picked[1] = high; s.picked[2] = (uint32_t)s.n; }
+        }
+        __syncthreads();
+        largest = s.picked[1];
+        return s.picked[0];
+    }
+
+    // The logits of a thread's chunks j0, j0 + kThreads, ... that reach the bound, into the list.
+    __device__ __forceinline__ void take(const Chunk<T> (&c)[kBatch], int j0, float bound) {
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int j = j0 + x * kThreads;
+            if (j >= nvec || !(c[x].most() >= bound)) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (c[x].raw_at(e) >= bound) put(c[x].raw_at(e), base + j * N + e);
+        }
+    }
+    // Drops the list's entries below a key. Not for a list that has overflowed.
+    __device__ __forceinline__ void drop_below(uint32_t key) {
+        constexpr int PER = kCap / kThreads;
+        u64 e[PER];
+        __syncthreads();
+        const int n = s.n;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            e[j] = i < n ? s.list[i] : 0;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (e[j] && (uint32_t)(e[j] >> 32) >= key) s.list[atomicAdd(&s.n, 1)] = e[j];
+        __syncthreads();
+    }
+
+    // Streams the slice and leaves every logit that can be among the row's k largest in the CTAs' lists (or more than
+    // kCap in one, which says that the list will not do). Sets `top`.
+    __device__ __forceinline__ void stream(int k) {
+        const int share = (k + ranks - 1) / ranks;  // so many of every CTA together are k
+        float most[2] = {-INFINITY, -INFINITY};
+        uint32_t largest, own = 0;
+        if (threadIdx.x == 0) s.n = 0;
+        Chunk<T> c[kBatch];
+        auto fetch = [&](Chunk<T> (&to)[kBatch], int j0) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x)
+                if (j0 + x * kThreads < nvec) to[x] = load_global(j0 + x * kThreads);
+        };
+        auto look = [&](int j0) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x)
+                if (j0 + x * kThreads < nvec) most[x & 1] = fmaxf(most[x & 1], c[x].most());
+        };
+        constexpr int kStep = kBatch * kThreads;
+        fetch(c, threadIdx.x);
+        const bool one = nvec <= kStep;
+        if (!one) {
+            int renew = kStep;  // chunks seen at the next renewal of the bound
+            float bound = kLowest;
+            for (int j0 = threadIdx.x, seen = kStep; ; j0 += kStep, seen += kStep) {
+                Chunk<T> next[kBatch];
+                if (seen < nvec) fetch(next, j0 + kStep);
+                look(j0);
+                if (seen >= renew || seen >= nvec) {
+                    own = select(most, k, largest);
+                    bound = bound_of(own);
+                    renew = 2 * seen;
+                    const int n = (int)s.picked[2];  // s.n itself is on the move again
+                    if (n > kCap / 2 && n <= kCap) drop_below(own);
+                }
+                take(c, j0, bound);
+                if (seen >= nvec) break;
+#pragma unroll
+                for (int x = 0; x < kBatch; ++x) c[x].raw = next[x].raw;
+            }
+            __syncthreads();
+        } else {
+            look(threadIdx.x);
+        }
+        uint32_t bound = one || ranks > 1 ? select(most, share, largest) : own;
+        const u64 o = exchange((u64)largest << 32 | bound);
+        const bool lane_in = (threadIdx.x & 31) < ranks;
+        top = value_of(__reduce_max_sync(0xffffffffu, (uint32_t)(o >> 32)));
+        bound = max(own, __reduce_min_sync(0xffffffffu, lane_in ? (uint32_t)o : 0xffffffffu));
+        if (one) take(c, threadIdx.x, bound_of(bound));
+        else if (s.n <= kCap) drop_below(bound);
+    }
+
+    // Reads the slice for the general way (and keeps it in shared memory, if it fits). Sets `top`.
+    __device__ __forceinline__ void read_slice() {
+        float most = -INFINITY;
+        for (int j0 = threadIdx.x; j0 < nvec; j0 += kBatch * kThreads) {
+            Chunk<T> c[kBatch];
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x)
+                if (j0 + x * kThreads < nvec) c[x] = load_global(j0 + x * kThreads);
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) {
+                if (j0 + x * kThreads >= nvec) continue;
+                if (staged) reinterpret_cast<uint4*>(stage)[j0 + x * kThreads] = c[x].raw;
+                most = fmaxf(most, c[x].most());
+            }
+        }
+        uint32_t key = __reduce_max_sync(0xffffffffu, key_of(most));
+        if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = key;
+        __syncthreads();
+        key = __reduce_max_sync(0xffffffffu, (uint32_t)s.part[threadIdx.x & (kWarps - 1)]);
+        top = value_of(__reduce_max_sync(0xffffffffu, (uint32_t)exchange(key)));
+    }
+
+    __device__ __forceinline__ void greedy(int64_t* token) {
+        uint32_t first = 0x7fffffffu;
+        each([&](float v, int i) { if (v == top) first = min(first, (uint32_t)i); });
+        first = __reduce_min_sync(0xffffffffu, first);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = first;
+        __syncthreads();
+        first = __reduce_min_sync(0xffffffffu, (uint32_t)s.part[threadIdx.x & (kWarps - 1)]);
+        const uint32_t o = (uint32_t)exchange(first);
+        first = __reduce_min_sync(0xffffffffu, (threadIdx.x & 31) < ranks ? o : 0xffffffffu);
+        if (rank == 0 && threadIdx.x == 0) *token = (int64_t)first;
+    }
 };
 
-template <typename T, bool STAGED>
-__global__ void __launch_bounds__(kThreads, STAGED ? 2 : 1) sample_kernel(const SampleParams P) {
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams P) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
     extern __shared__ __align__(16) unsigned char stage[];
     __shared__ Shared shared;
     auto cluster = cg::this_cluster();
-    using R = Row<T, STAGED>;
+    using R = Row<T>;
     constexpr int N = R::N;
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    auto started = cluster.barrier_arrive();  // the first exchange writes to CTAs that must have started
     const int64_t b = blockIdx.x / ranks;
     const T* row = (const T*)P.logits + b * P.row_stride;
     const int lo = min(P.vocab, rank * P.slice), hi = min(P.vocab, lo + P.slice);
     const int phase = (int)(((uintptr_t)(row + lo) & 15) / sizeof(T));
-    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0};
-    r.vocab = P.vocab;
+    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0, P.vocab, false};
 
     const float temperature = P.temperature ? P.temperature[b] : P.temperature0;
     const float p = P.top_p ? P.top_p[b] : P.top_p0, min_p = P.min_p ? P.min_p[b] : P.min_p0;
@@ -510,90 +776,38 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 2 : 1) sample_kernel(const 
     if (k <= 0 || k > P.vocab) k = P.vocab;
     const float u = P.u[b];
     int64_t* token = P.tokens + b;
+    const bool greedy = !(temperature > 0.f), by_list = !greedy && k < P.vocab && k <= kListK;
 
-    // the slice into shared memory; the thread's largest logit on the way
-    uint32_t most = 0;
-    for (int j0 = threadIdx.x; j0 < r.nvec; j0 += 4 * kThreads) {
-        Chunk<T> c[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            if (j0 + x * kThreads < r.nvec) c[x] = r.load_global(j0 + x * kThreads);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int j = j0 + x * kThreads;
-            if (j >= r.nvec) continue;
-            if (STAGED) reinterpret_cast<uint4*>(stage)[j] = c[x].raw;
-#pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int i = r.base + j * N + e;
-                if (i >= lo && i < hi) most = max(most, key_of(c[x].at(e)));
-            }
-        }
-    }
-    const bool greedy = !(temperature > 0.f);
-    const int local = (k + ranks - 1) / ranks;
-    const bool by_list = !greedy && k < P.vocab && local <= kThreads;
-    uint32_t bound = 0;  // at least `local` threads hold a logit with a key from here on
-    if (by_list) {
-        for (int bit = 31; bit >= 10; --bit)
-            if (__syncthreads_count(most >= (bound | 1u << bit)) >= local) bound |= 1u << bit;
-    }
-    __syncthreads();
-    {
-        uint32_t top = most;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((threadIdx.x & 31) == 0) shared.part[threadIdx.x >> 5] = top;
-        __syncthreads();
-        for (int w = 0; w < kWarps; ++w) top = max(top, (uint32_t)shared.part[w]);
-        u64* slot = r.exchange((u64)top << 32 | bound);
-        for (int x = 0; x < ranks; ++x) {
-            const u64 o = r.word(slot, x);
-            top = max(top, (uint32_t)(o >> 32));
-            bound = min(bound, (uint32_t)o);
-        }
-        r.top = value_of(top);
-    }
-    r.scale = fmax(1.0 / (double)temperature, 1e-300);  // at T = inf every finite logit weighs 1
+    r.scale = fmax(1.4426950408889634 / (double)temperature, 1e-300);  // at T = inf every finite logit weighs 1
+    r.shift = P.shift;
     r.unit = (double)(1ull << P.shift);
     r.bins = (float)((double)kBins / (((double)P.shift + 2.0) * 0.6931471805599453 * (double)temperature));
     r.cut_key = 0;
     r.cut_index = 0;
+    cluster.barrier_wait(std::move(started));
 
-    if (r.top == -INFINITY) {  // nothing to draw from
-        if (rank == 0 && threadIdx.x == 0) *token = -1;
-    } else if (greedy) {
-        int first = 0x7fffffff;
-        r.each([&](float v, int i) { if (v == r.top) first = min(first, i); });
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) shared.part[threadIdx.x >> 5] = (u64)first;
-        __syncthreads();
-        u64 least = shared.part[0];
-        for (int w = 1; w < kWarps; ++w) least = least < shared.part[w] ? least : shared.part[w];
-        u64* slot = r.exchange(least);
-        if (rank == 0 && threadIdx.x == 0) {
-            for (int x = 1; x < ranks; ++x) { const u64 o = r.word(slot, x); least = least < o ? least : o; }
-            *token = (int64_t)least;
+    if (by_list) {
+        r.stream(k);
+        const int n = r.top == -INFINITY ? 0 : r.collect();
+        if (r.top > -INFINITY && n <= kCap) {
+            // rank 0 has pulled the lists: the others may leave
+            auto pulled = cluster.barrier_arrive();
+            if (rank == 0) r.finish_list(n, k, p, min_p, u, token);
+            cluster.barrier_wait(std::move(pulled));
+            return;
         }
     } else {
-        bool done = false;
-        if (by_list) {
-            const uint32_t from = bound;
-            const int n = r.gather([&](float v, int) { return v > -INFINITY && key_of(v) >= from; });
-            if (n <= kCap) {
-                done = true;
-                if (rank == 0) r.finish_list(n, k, p, min_p, u, token);
-            }
-        }
-        if (!done) {
-            if (k < P.vocab) r.template cut<false>(k, 0.f);
-            if (p < 1.f) r.template cut<true>(0, p);
-            r.draw(u, min_p, token);
-        }
+        r.staged = P.staged != 0;
+        r.read_slice();
     }
-    cluster.sync();  // nobody leaves while its shared memory may still be read
+    if (r.top == -INFINITY) {  // nothing to draw from
+        if (rank == 0 && threadIdx.x == 0) *token = -1;
+        return;
+    }
+    if (greedy) return r.greedy(token);
+    if (k < P.vocab) r.template cut<false>(k, 0.f);
+    if (p < 1.f) r.template cut<true>(0, p);
+    r.draw(u, min_p, token);
 }
 
 }  // namespace
@@ -614,20 +828,19 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
 
-    // CTAs of a row: as many as its slice needs to leave room for a second CTA on the SM, and more while SMs would
-    // stand idle and a CTA keeps 8 logits or more a thread.
+    // CTAs of a row: one where the rows fill the GPU, else as many as fill it while a CTA keeps 8 logits or more a thread,
+    // and more for a slice that then stays in shared memory.
     int C = 1;
     auto slice_of = [&](int c) { return round_up<int64_t>(ceil_div<int64_t>(a->vocab, c), 8); };
-    while (C < kMaxCluster && ((slice_of(C) + 8) * e > kStageTwo || (a->batch * C < sm_count() && slice_of(C) > 8 * kThreads)))
-        C *= 2;
+    while (C < kMaxCluster && a->batch * C < sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
     const int64_t slice = slice_of(C);
     const size_t bytes = round_up<size_t>((size_t)(slice + 8) * e, 16);
-    const bool staged = bytes <= kStageMax;
+    const bool staged = bytes <= (a->batch * C > sm_count() ? kStageTwo : kStageMax);
     SampleParams P = {};
     P.logits = a->logits; P.u = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p;
     P.top_k = a->top_k; P.tokens = a->tokens; P.row_stride = a->row_stride;
     P.temperature0 = a->temperature_all; P.top_p0 = a->top_p_all; P.min_p0 = a->min_p_all; P.top_k0 = a->top_k_all;
-    P.vocab = (int)a->vocab; P.slice = (int)slice;
+    P.vocab = (int)a->vocab; P.slice = (int)slice; P.staged = staged ? 1 : 0;
     int log2v = 0;
     while ((1ll << log2v) < a->vocab) ++log2v;
     P.shift = 62 - log2v < 50 ? 62 - log2v : 50;
@@ -658,8 +871,7 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     };
     RFX_DISPATCH_DTYPE(a->dtype, T, {
         static PerDeviceOnce once;
-        if (staged) launch(sample_kernel<T, true>, once);
-        else launch(sample_kernel<T, false>, once);
+        launch(sample_kernel<T>, once);
     });
     if (le != cudaSuccess) { cudaGetLastError(); return fail(RFX_CUDA_ERROR, "%s: %s", name, cudaGetErrorString(le)); }
     return check_launch(name);
