@@ -26,6 +26,7 @@
 // three cluster barriers of a row in small ones; general rows by the 64-bit exponentials, one a logit.
 #include <cooperative_groups.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "common.cuh"
@@ -39,7 +40,7 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCap = 2048;     // logits that one CTA ranks
-constexpr int kPairs = 512;    // up to here by comparing all pairs, behind by sorting
+constexpr int kPairs = 128;    // up to here by comparing all pairs, behind by sorting
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 2 * kThreads;     // groups whose maxima bound the k-th largest logit
@@ -98,15 +99,15 @@ template <typename T> struct Chunk {  // 16 bytes of logits
         return f == f ? f : -INFINITY;  // NaN counts as masked
     }
     __device__ __forceinline__ float raw_at(int e) const { return Num<T>::to_f(v[e]); }
-    // The largest that is no NaN; -inf if all are.
+    // The largest that is no NaN; NaN if all are.
     __device__ __forceinline__ float most() const {
         if constexpr (sizeof(T) == 4) {
-            return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), -INFINITY);
+            return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
         } else {
             using W = typename Pair16<T>::P;
             const W* w = reinterpret_cast<const W*>(v);
             const float2 f = Pair16<T>::widen(__hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3])));
-            return fmaxf(fmaxf(f.x, f.y), -INFINITY);
+            return fmaxf(f.x, f.y);
         }
     }
 };
@@ -131,6 +132,103 @@ __device__ __noinline__ void sort_list(u64* list, int n) {
     __syncthreads();
 }
 
+// Sorts list[0, n), falling, by bins: bin(entry) in [0, kBins) never falls while entries fall. An entry's place is its
+// bin's first place and the number of larger entries in the bin, so the cost is a dozen barriers and a few steps per
+// entry (300 entries: 1 us; the bitonic network's 45 stages 3 us). A bin of more than 64 entries leaves it to the network.
+template <typename F> __device__ __forceinline__ void sort_by_bins(Shared& s, int n, F bin) {
+    constexpr int PER = kCap / kThreads;
+    __syncthreads();
+    reinterpret_cast<uint4*>(s.hist.lo)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    u64 e[PER];
+    int b[PER], at[PER];
+    bool crowded = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int i = threadIdx.x + j * kThreads;
+        e[j] = 0;
+        if (i >= n) continue;
+        e[j] = s.list[i];
+        b[j] = bin(e[j]);
+        at[j] = (int)atomicAdd(&s.hist.lo[b[j]], 1u);
+        crowded |= at[j] >= 64;
+    }
+    if (__syncthreads_or(crowded)) return sort_list(s.list, n);
+    const uint4 m = reinterpret_cast<const uint4*>(s.hist.lo)[threadIdx.x];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t own = m.x + m.y + m.z + m.w;
+    uint32_t x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s.part[warp] = x;
+    __syncthreads();
+    const uint32_t ahead = __reduce_add_sync(0xffffffffu, lane < warp ? (uint32_t)s.part[lane & (kWarps - 1)] : 0u);
+    uint4 first;
+    first.x = ahead + x - own; first.y = first.x + m.x; first.z = first.y + m.y; first.w = first.z + m.z;
+    reinterpret_cast<uint4*>(s.hist.lo)[threadIdx.x] = first;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (e[j]) s.list[s.hist.lo[b[j]] + at[j]] = e[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (!e[j]) continue;
+        const int from = (int)s.hist.lo[b[j]], to = (int)(b[j] + 1 < kBins ? s.hist.lo[b[j] + 1] : (uint32_t)n);
+        int place = from;
+        for (int i = from; i < to; ++i) place += s.list[i] > e[j];
+        at[j] = place;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (e[j]) s.list[at[j]] = e[j];
+    __syncthreads();
+}
+
+// A key that at least `count` <= kGroups of the CTA's group maxima reach (a key of -inf or below, if fewer groups hold
+// logits): the count-th largest with its last bits cleared, ten bits below the highest in which two maxima differ.
+// Leaves it, the largest key and s.n in s.picked. One histogram over those ten bits and a scan: four barriers.
+// (One warp that searched bit by bit took 2 us.)
+__device__ __forceinline__ void select(Shared& s, float most0, float most1, int count) {
+    static_assert(kGroups == 1024 && kThreads == 512, "ten bits, two bins a thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t k0 = key_of(most0), k1 = key_of(most1);
+    reinterpret_cast<uint2*>(s.group)[threadIdx.x] = make_uint2(0, 0);
+    const uint32_t h = __reduce_max_sync(0xffffffffu, max(k0, k1)), l = __reduce_min_sync(0xffffffffu, min(k0, k1));
+    if (lane == 0) s.part[warp] = (u64)h << 32 | l;
+    __syncthreads();
+    const u64 hl = s.part[lane & (kWarps - 1)];
+    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(hl >> 32));
+    const uint32_t low = __reduce_min_sync(0xffffffffu, (uint32_t)hl);
+    const int first = high == low ? 0 : 31 - __clz(high ^ low), shift = max(0, first - 9);
+    const uint32_t base = first == 31 ? 0 : high >> (first + 1) << (first + 1);
+    atomicAdd(&s.group[1023 - ((k0 - base) >> shift)], 1u);  // the largest in front
+    atomicAdd(&s.group[1023 - ((k1 - base) >> shift)], 1u);
+    if (threadIdx.x == 0) { s.picked[1] = high; s.picked[2] = (uint32_t)s.n; }
+    __syncthreads();
+    const uint2 m = reinterpret_cast<const uint2*>(s.group)[threadIdx.x];
+    const int own = (int)(m.x + m.y);
+    int x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s.part[warp] = (u64)x;
+    __syncthreads();
+    const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? (int)s.part[lane & (kWarps - 1)] : 0);
+    const int before = ahead + x - own;
+    if (before < count && before + own >= count) {
+        const uint32_t bin = 2 * threadIdx.x + (before + (int)m.x >= count ? 0 : 1);
+        s.picked[0] = base + ((1023 - bin) << shift);
+    }
+    __syncthreads();
+}
+
 // One CTA's view of its row.
 template <typename T> struct Row {
     static constexpr int N = Chunk<T>::N;
@@ -150,16 +248,43 @@ template <typename T> struct Row {
     uint32_t cut_key;     // kept: key > cut_key, or key == cut_key and index <= cut_index
     int cut_index;
 
-    __device__ __forceinline__ Chunk<T> load_global(int j) const {
+    // A chunk that reaches over an end of the slice (the first or the last one), element by element.
+    __device__ __forceinline__ Chunk<T> load_edge(int j) const {
         Chunk<T> c;
         const int i0 = base + j * N;
-        if (i0 >= lo && i0 + N <= hi) {
-            c.raw = __ldg(reinterpret_cast<const uint4*>(row + i0));
-        } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) c.v[e] = i0 + e >= lo && i0 + e < hi ? row[i0 + e] : Num<T>::from_f(-INFINITY);
-        }
+        for (int e = 0; e < N; ++e) c.v[e] = i0 + e >= lo && i0 + e < hi ? row[i0 + e] : Num<T>::from_f(-INFINITY);
         return c;
+    }
+    __device__ __forceinline__ bool whole(int j) const { return base + j * N >= lo && base + j * N + N <= hi; }
+    __device__ __forceinline__ Chunk<T> load_global(int j) const {
+        Chunk<T> c;
+        if (!whole(j)) return load_edge(j);
+        c.raw = __ldg(reinterpret_cast<const uint4*>(row + base + j * N));
+        return c;
+    }
+    // Whether the kBatch * kThreads chunks from j on are all whole.
+    __device__ __forceinline__ bool inside(int j) const { return whole(j) && j + kBatch * kThreads <= nvec && whole(j + kBatch * kThreads - 1); }
+    // Chunks j0, j0 + kThreads, ...: all loads go out before anything waits for one of them. A branch around each
+    // (the ends of the slice) made them wait for one another, so where a batch is not inside the slice they are
+    // loaded from the nearest whole chunk first and replaced afterwards. Chunks behind the last hold anything.
+    template <bool INSIDE> __device__ __forceinline__ void fetch(Chunk<T> (&to)[kBatch], int j0) const {
+        const uint4* from = reinterpret_cast<const uint4*>(row + base);
+        if (INSIDE) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) to[x].raw = __ldg(from + j0 + x * kThreads);
+            return;
+        }
+        const int first = whole(0) ? 0 : 1, last = whole(nvec - 1) ? nvec - 1 : nvec - 2;
+        if (first <= last) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) to[x].raw = __ldg(from + max(first, min(last, j0 + x * kThreads)));
+        }
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int j = j0 + x * kThreads;
+            if (j < nvec && (j < first || j > last)) to[x] = load_edge(j);
+        }
     }
     __device__ __forceinline__ Chunk<T> load(int j) const {
         if (!staged) return load_global(j);
@@ -370,7 +495,13 @@ template <typename T> struct Row {
                         if (before < target && before + m >= target) s.found[0] = e;
                     });
                 } else {
-                    sort_list(s.list, n);
+                    const float low = value_of(__reduce_min_sync(0xffffffffu, lowest_key(n)));
+                    const float high = top - (bins > 0.f ? (float)bin / bins : 0.f);
+                    const float per_unit = high - low > 0.f ? (float)(kBins - 1) / fminf(high - low, 3.4e38f) : 0.f;
+                    sort_by_bins(s, n, [&](u64 e) {
+                        const float d = high - value_of((uint32_t)(e >> 32));
+                        return d > 0.f ? min(kBins - 1, (int)(fminf(d, 3.4e38f) * per_unit)) : 0;
+                    });
                     constexpr int PER = kCap / kThreads;
                     u64 m[PER], sum = 0, total;
 #pragma unroll
@@ -527,31 +658,39 @@ template <typename T> struct Row {
             const u64 total = block_sum(in ? m : 0);  // (its barrier also ends the reading of s.pair)
             if (p < 1.f) in = in && before < target_of(p, total);
             in = in && weight(value_of((uint32_t)(key >> 32))) >= least;
-            if (!in) m = 0;
-            const u64 sum = block_sum(m);
-            if (threadIdx.x < n) s.pair[threadIdx.x] = Entry{key << 32, m};  // falling in ~index: rising in index
+            if (threadIdx.x < n) s.pair[threadIdx.x] = Entry{key << 32, in ? m : 0};  // falling in ~index: rising in index
             __syncthreads();
-            if (!in) return;
-            u64 at = 0;
-            key <<= 32;
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) {
-                const Entry o = s.pair[j];
-                if (o.key > key) at += o.mass;
-            }
-            const u64 x = drawn(u, sum);
-            if (x >= at && x < at + m) *token = (int64_t)(0xffffffffu - (uint32_t)(key >> 32));
-            return;
+            return draw_pairs(n, u, token);
         }
-        sort_list(s.list, n);
-        if (k < n) n = k;
-        constexpr int PER = kCap / kThreads;
-        u64 m[PER], sum = 0, total;
+        // falling from the largest to the smallest listed
+        const float low = value_of(__reduce_min_sync(0xffffffffu, lowest_key(n)));
+        const float per_unit = top - low > 0.f ? (float)(kBins - 1) / fminf(top - low, 3.4e38f) : 0.f;
+        sort_by_bins(s, n, [&](u64 e) {
+            const float d = top - value_of((uint32_t)(e >> 32));
+            return d > 0.f ? min(kBins - 1, (int)(fminf(d, 3.4e38f) * per_unit)) : 0;
+        });
+        if (min(n, k) <= kThreads) finish_sorted<1>(min(n, k), p, least, u, token);
+        else finish_sorted<kCap / kThreads>(min(n, k), p, least, u, token);
+    }
+    // The smallest key of list[0, n), over the whole CTA, in every lane.
+    __device__ __forceinline__ uint32_t lowest_key(int n) {
+        uint32_t low = 0xffffffffu;
+        for (int i = threadIdx.x; i < n; i += kThreads) low = min(low, (uint32_t)(s.list[i] >> 32));
+        low = __reduce_min_sync(0xffffffffu, low);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = low;
+        __syncthreads();
+        return (uint32_t)s.part[threadIdx.x & (kWarps - 1)];
+    }
+    // The rest over a sorted list of at most PER * kThreads entries, PER neighbours a thread.
+    template <int PER> __device__ __forceinline__ void finish_sorted(int n, float p, double least, float u, int64_t* token) {
+        u64 m[PER], e[PER], sum = 0, total;
         double w[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x * PER + j;
-            w[j] = i < n ? weight(value_of((uint32_t)(s.list[i] >> 32))) : -1.0;
+            e[j] = i < n ? s.list[i] : 0;
+            w[j] = i < n ? weight(value_of((uint32_t)(e[j] >> 32))) : -1.0;
             m[j] = i < n ? fixed(w[j]) : 0;
             sum += m[j];
         }
@@ -566,20 +705,30 @@ template <typename T> struct Row {
             stay += in;
         }
         const int kept_n = (int)block_sum((u64)stay);  // a prefix of the list: weights only fall
-        // in index order: entries (index, place), with their weights beside them
-        u64 e[PER];
+        if (kept_n <= kPairs) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            e[j] = i < kept_n ? (s.list[i] << 32 | (u64)i) : 0;  // low word: ~index, so falling is rising in index
+            for (int j = 0; j < PER; ++j) {
+                const int i = threadIdx.x * PER + j;
+                if (i < kept_n) s.pair[i] = Entry{e[j] << 32, m[j]};  // falling in ~index: rising in index
+            }
+            __syncthreads();
+            return draw_pairs(kept_n, u, token);
         }
+        // in index order: entries (index, place), with their weights beside them
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x * PER + j;
-            if (i < kept_n) { s.list[i] = e[j]; s.weight[i] = m[j]; }
+            if (i < kept_n) s.list[i] = e[j] << 32 | (u64)i;
         }
-        sort_list(s.list, kept_n);
+        const float per_index = (float)(kBins - 1) / (float)vocab;
+        sort_by_bins(s, kept_n, [&](u64 x) { return (int)((float)(0xffffffffu - (uint32_t)(x >> 32)) * per_index); });
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x * PER + j;
+            if (i < kept_n) s.weight[i] = m[j];
+        }
+        __syncthreads();
         sum = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -596,53 +745,42 @@ template <typename T> struct Row {
             at += m[j];
         }
     }
-
-    // A key that at least `count` of the CTA's group maxima reach (0 if there are fewer groups with logits), within 2^-10 of the
-    // spread of the maxima's bits below the count-th; and their largest key. One warp searches, bit by bit.
-    __device__ __forceinline__ uint32_t select(const float (&most)[2], int count, uint32_t& largest) {
-        s.group[threadIdx.x] = key_of(most[0]);
-        s.group[kThreads + threadIdx.x] = key_of(most[1]);
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            uint32_t k[kGroups / 32], high = 0, low = 0xffffffffu;
-#pragma unroll
-            for (int x = 0; x < kGroups / 128; ++x) {
-                const uint4 v = reinterpret_cast<const uint4*>(s.group)[x * 32 + threadIdx.x];
-                k[4 * x] = v.x; k[4 * x + 1] = v.y; k[4 * x + 2] = v.z; k[4 * x + 3] = v.w;
-            }
-#pragma unroll
-            for (int x = 0; x < kGroups / 32; ++x) { high = max(high, k[x]); low = min(low, k[x]); }
-            high = __reduce_max_sync(0xffffffffu, high);
-            low = __reduce_min_sync(0xffffffffu, low);
-            uint32_t bound = high;
-            if (high != low) {
-                const int first = 31 - __clz(high ^ low);
-                bound = first == 31 ? 0 : high >> (first + 1) << (first + 1);
-                for (int bit = first; bit >= max(0, first - 9); --bit) {
-                    const uint32_t next = bound | 1u << bit;
-                    int c = 0;
-#pragma unroll
-                    for (int x = 0; x < kGroups / 32; ++x) c += k[x] >= next;
-                    if (__reduce_add_sync(0xffffffffu, c) >= count) bound = next;
-                }
-            }
-            if (threadIdx.x == 0) { s.picked[0] = bound; s.picked[1] = high; s.picked[2] = (uint32_t)s.n; }
+    // The draw among pair[0, n): keys that fall as the index rises, and masses. Entry i belongs to thread i.
+    __device__ __forceinline__ void draw_pairs(int n, float u, int64_t* token) {
+        if (threadIdx.x >= n) return;
+        const Entry mine = s.pair[threadIdx.x];
+        u64 at = 0, sum = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const Entry o = s.pair[j];
+            if (o.key > mine.key) at += o.mass;
+            sum += o.mass;
         }
-        __syncthreads();
-        largest = s.picked[1];
-        return s.picked[0];
+        const u64 x = drawn(u, sum);
+        if (x >= at && x < at + mine.mass) *token = (int64_t)(0xffffffffu - (uint32_t)(mine.key >> 32));
     }
 
-    // The logits of a thread's chunks j0, j0 + kThreads, ... that reach the bound, into the list.
-    __device__ __forceinline__ void take(const Chunk<T> (&c)[kBatch], int j0, float bound) {
+    // The logits of a thread's chunks j0, j0 + kThreads, ... that reach the bound, into the list. Few threads have one, so
+    // which they are is found first, then one atomic makes room for them and they are read once more (from L1).
+    template <bool INSIDE> __device__ __forceinline__ void take(const Chunk<T> (&c)[kBatch], int j0, float bound) {
+        uint32_t in = 0;
 #pragma unroll
         for (int x = 0; x < kBatch; ++x) {
-            const int j = j0 + x * kThreads;
-            if (j >= nvec || !(c[x].most() >= bound)) continue;
+            if (!(c[x].most() >= bound)) continue;
+            if (!INSIDE && j0 + x * kThreads >= nvec) continue;
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (c[x].raw_at(e) >= bound) put(c[x].raw_at(e), base + j * N + e);
+                if (c[x].raw_at(e) >= bound) in |= 1u << (x * N + e);
         }
+        if (!in) return;
+        int at = atomicAdd(&s.n, __popc(in));
+        do {
+            const int bit = __ffs(in) - 1;
+            in &= in - 1;
+            const int i = base + (j0 + bit / N * kThreads) * N + bit % N;
+            if (at < kCap) s.list[at] = (u64)key_of(Num<T>::to_f(row[i])) << 32 | (0xffffffffu - (uint32_t)i);
+            ++at;
+        } while (in);
     }
     // Drops the list's entries below a key. Not for a list that has overflowed.
     __device__ __forceinline__ void drop_below(uint32_t key) {
@@ -669,51 +807,57 @@ template <typename T> struct Row {
     __device__ __forceinline__ void stream(int k) {
         const int share = (k + ranks - 1) / ranks;  // so many of every CTA together are k
         float most[2] = {-INFINITY, -INFINITY};
-        uint32_t largest, own = 0;
+        uint32_t own = 0;
         if (threadIdx.x == 0) s.n = 0;
         Chunk<T> c[kBatch];
-        auto fetch = [&](Chunk<T> (&to)[kBatch], int j0) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x)
-                if (j0 + x * kThreads < nvec) to[x] = load_global(j0 + x * kThreads);
-        };
-        auto look = [&](int j0) {
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x)
-                if (j0 + x * kThreads < nvec) most[x & 1] = fmaxf(most[x & 1], c[x].most());
-        };
         constexpr int kStep = kBatch * kThreads;
-        fetch(c, threadIdx.x);
+        auto look = [&](const Chunk<T> (&c)[kBatch], int j0, auto inside) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x)
+                if (inside || j0 + x * kThreads < nvec) most[x & 1] = fmaxf(most[x & 1], c[x].most());
+        };
+        const std::integral_constant<bool, false> ends;
+        const std::integral_constant<bool, true> whole_batch;
         const bool one = nvec <= kStep;
-        if (!one) {
-            int renew = kStep;  // chunks seen at the next renewal of the bound
+        if (one) {
+            fetch<false>(c, threadIdx.x);
+            look(c, threadIdx.x, ends);
+        } else {
             float bound = kLowest;
-            for (int j0 = threadIdx.x, seen = kStep; ; j0 += kStep, seen += kStep) {
-                Chunk<T> next[kBatch];
-                if (seen < nvec) fetch(next, j0 + kStep);
-                look(j0);
+            int j0 = threadIdx.x, seen = kStep, renew = kStep;  // renew: chunks seen when the bound is renewed next
+            bool here = inside(0);
+            if (here) fetch<true>(c, j0); else fetch<false>(c, j0);
+            auto batch = [&](const Chunk<T> (&c)[kBatch], Chunk<T> (&next)[kBatch]) {
+                const bool there = seen < nvec && inside(seen);
+                if (there) fetch<true>(next, j0 + kStep);
+                else if (seen < nvec) fetch<false>(next, j0 + kStep);
+                if (here) look(c, j0, whole_batch); else look(c, j0, ends);
                 if (seen >= renew || seen >= nvec) {
-                    own = select(most, k, largest);
+                    select(s, most[0], most[1], k);
+                    own = s.picked[0];
                     bound = bound_of(own);
                     renew = 2 * seen;
                     const int n = (int)s.picked[2];  // s.n itself is on the move again
                     if (n > kCap / 2 && n <= kCap) drop_below(own);
                 }
-                take(c, j0, bound);
-                if (seen >= nvec) break;
-#pragma unroll
-                for (int x = 0; x < kBatch; ++x) c[x].raw = next[x].raw;
-            }
+                if (here) take<true>(c, j0, bound); else take<false>(c, j0, bound);
+                if (seen >= nvec) return false;
+                here = there;
+                j0 += kStep;
+                seen += kStep;
+                return true;
+            };
+            Chunk<T> other[kBatch];
+            while (batch(c, other) && batch(other, c)) {}
             __syncthreads();
-        } else {
-            look(threadIdx.x);
         }
-        uint32_t bound = one || ranks > 1 ? select(most, share, largest) : own;
-        const u64 o = exchange((u64)largest << 32 | bound);
+        if (one || ranks > 1) select(s, most[0], most[1], share);
+        uint32_t bound = s.picked[0];
+        const u64 o = exchange((u64)s.picked[1] << 32 | bound);
         const bool lane_in = (threadIdx.x & 31) < ranks;
         top = value_of(__reduce_max_sync(0xffffffffu, (uint32_t)(o >> 32)));
         bound = max(own, __reduce_min_sync(0xffffffffu, lane_in ? (uint32_t)o : 0xffffffffu));
-        if (one) take(c, threadIdx.x, bound_of(bound));
+        if (one) take<false>(c, threadIdx.x, bound_of(bound));
         else if (s.n <= kCap) drop_below(bound);
     }
 
@@ -722,9 +866,7 @@ template <typename T> struct Row {
         float most = -INFINITY;
         for (int j0 = threadIdx.x; j0 < nvec; j0 += kBatch * kThreads) {
             Chunk<T> c[kBatch];
-#pragma unroll
-            for (int x = 0; x < kBatch; ++x)
-                if (j0 + x * kThreads < nvec) c[x] = load_global(j0 + x * kThreads);
+            if (inside(j0 - threadIdx.x)) fetch<true>(c, j0); else fetch<false>(c, j0);
 #pragma unroll
             for (int x = 0; x < kBatch; ++x) {
                 if (j0 + x * kThreads >= nvec) continue;
