@@ -338,7 +338,7 @@ int rfx_online_softmax(const RfxSoftmaxArgs* a);
  *   min_p: w >= min(min_p, 1) stays, the largest w being 1 (min_p <= 0 or NaN: all);
  *   token = the lowest index at which the running sum of the staying w, in index order, exceeds
  *   uniform * their sum (uniform >= 1: the last of weight, below 0 or NaN: the first).
- * temperature <= 0 or NaN: the lowest index of the largest logit. A row with nothing but -inf (or NaN) gives
+ * temperature <= 0 or NaN: the lowest index of the largest logit (above 0 it counts as 1e-20 at least). A row with nothing but -inf (or NaN) gives
  * -1; with +inf among its logits those share the mass. Every setting is a device array [batch], or with a
  * NULL pointer one number for all rows. Weights are exp in 64 bits, summed as whole multiples of 2^-S of the
  * largest, S = min(50, 62 - log2 vocab): the result depends on nothing but the arguments. vocab <= 2^24. */

@@ -26,6 +26,8 @@
 // three cluster barriers of a row in small ones; general rows by the 64-bit exponentials, one a logit.
 #include <cooperative_groups.h>
 
+#include <math.h>
+
 #include <type_traits>
 #include <utility>
 
@@ -41,7 +43,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCap = 2048;     // logits that one CTA ranks
 constexpr int kPairs = 128;    // up to here by comparing all pairs, behind by sorting
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;   // more than 32 * (S + 2), the steps to a weight of zero
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 2 * kThreads;     // groups whose maxima bound the k-th largest logit
 constexpr int kListK = kGroups / 2;       // with k near kGroups the bound sinks to the smallest of the maxima
@@ -60,6 +62,7 @@ struct SampleParams {
     int32_t top_k0;
     int vocab, slice;  // slice: logits per CTA, a multiple of 8
     int shift;         // S: weights are multiples of 2^-S
+    double power[32];  // 2^(i/32)
     int staged;        // general rows keep their slice in shared memory
 };
 
@@ -75,7 +78,8 @@ struct __align__(16) Shared {
     };
     u64 part[kWarps];
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
-    u64 found[3];              // what rank 0 tells everyone
+    u64 found[3];              // what one CTA tells all: a bin and the sum before it, a cut
+    double power[32];          // 2^(i/32)
     uint32_t picked[3];        // of select(): the bound, the largest key, n before it
     int n;                     // entries that want to be in `list`
 };
@@ -229,6 +233,10 @@ __device__ __forceinline__ void select(Shared& s, float most0, float most1, int 
     __syncthreads();
 }
 
+// (ln 2 / 32)^k / k! for k = 1 .. 4
+__device__ constexpr double kTerm[4] = {0.02166084939249829, 0.00023459619820224677, 1.6938509724371819e-06, 9.172562701824643e-09};
+constexpr float kMagicF = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number
+
 // One CTA's view of its row.
 template <typename T> struct Row {
     static constexpr int N = Chunk<T>::N;
@@ -241,13 +249,19 @@ template <typename T> struct Row {
     int vocab;
     bool staged;
     float top;            // the row's largest logit
-    double scale;         // log2-weight per unit: log2(e) / T
-    double unit;          // 2^S
-    int shift;            // S
-    float bins;           // histogram bins per unit
-    uint32_t cut_key;     // kept: key > cut_key, or key == cut_key and index <= cut_index
+    float top_finite;     // the same, at most the largest finite float
+    float scale_f;        // 32 log2(e) / T
+    double top_wide, scale; // 32 log2 of a weight: (v - top) * scale
+    int shift, least_n;   // S; 32 log2 of a weight below which it is 0
+    float cut_value;      // kept: v > cut_value, or v == cut_value and index <= cut_index
     int cut_index;
 
+    __device__ __forceinline__ void set_top(float v) {
+        top = v;
+        top_finite = fminf(v, -kLowest);
+        if (v == INFINITY) scale_f = 1e30f;  // next to infinities nothing else weighs
+        top_wide = widen(v);
+    }
     // A chunk that reaches over an end of the slice (the first or the last one), element by element.
     __device__ __forceinline__ Chunk<T> load_edge(int j) const {
         Chunk<T> c;
@@ -292,6 +306,10 @@ template <typename T> struct Row {
         c.raw = reinterpret_cast<const uint4*>(stage)[j];
         return c;
     }
+    // f(chunk, index of its first logit) for the slice; what lies outside it reads as -inf
+    template <typename F> __device__ __forceinline__ void each_chunk(F f) const {
+        for (int j = threadIdx.x; j < nvec; j += kThreads) f(load(j), base + j * N);
+    }
     // f(value, index) for the slice; what lies outside it reads as -inf
     template <typename F> __device__ __forceinline__ void each(F f) const {
         for (int j = threadIdx.x; j < nvec; j += kThreads) {
@@ -300,45 +318,40 @@ template <typename T> struct Row {
             for (int e = 0; e < N; ++e) f(c.at(e), base + j * N + e);
         }
     }
-    // exp((v - top) / T) * 2^S, 0 where that is below a quarter. 2^t = 2^n * 2^f with n whole and |f| <= 1/2, and
-    // 2^f = sum (f ln 2)^k / k! to k = 12: the first term left out is below 2e-16 of the sum.
-    __device__ __forceinline__ double weight(float v) const {
-        const double t = v == top ? 0.0 : ((double)v - (double)top) * scale;
-        if (!(t >= -(double)(shift + 2))) return 0.0;
-        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-        const double n = t + kMagic;
-        const double f = t - (n - kMagic);
-        double w = 2.5678435993488196e-11;   // ln2^12 / 12!
-        w = fma(w, f, 4.44553827187081e-10);
-        w = fma(w, f, 7.054911620801121e-09);
-        w = fma(w, f, 1.0178086009239696e-07);
-        w = fma(w, f, 1.3215486790144305e-06);
-        w = fma(w, f, 1.5252733804059838e-05);
-        w = fma(w, f, 0.00015403530393381606);
-        w = fma(w, f, 0.0013333558146428441);
-        w = fma(w, f, 0.009618129107628477);
-        w = fma(w, f, 0.055504108664821576);
-        w = fma(w, f, 0.2402265069591007);
-        w = fma(w, f, 0.6931471805599453);
-        w = fma(w, f, 1.0);
-        const int e = __double2loint(n) + shift;
-        return __hiloint2double(__double2hiint(w) + (e << 20), __double2loint(w));
+    // A finite float as a double by moving its bits: the conversion instruction runs at a quarter of the rate of a
+    // multiplication. What is below the smallest normal float becomes zero, an infinity 2^128.
+    __device__ __forceinline__ static double widen(float v) {
+        const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
+        return __hiloint2double(m < 0x00800000u ? 0 : (int)((m >> 3) + 0x38000000u | (b & 0x80000000u)), (int)(b << 29));
     }
-    // To a whole number: below 2^52 the sum with 2^52 holds it in its low bits.
-    __device__ __forceinline__ u64 fixed(double w) const {
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+    // 32 log2 of the weight exp((v - top) / T), rounded to a whole number in fp32: also the histogram's bin, negated.
+    // Never rises as v falls; -4096 for NaN, -inf and all that is far below.
+    __device__ __forceinline__ float steps(float v) const { return fmaxf((fminf(v, -kLowest) - top_finite) * scale_f, -4096.f) + kMagicF; }
+    __device__ __forceinline__ static int whole_steps(float x) { return (int)__float_as_uint(x) - 0x4b400000; }
+    __device__ __forceinline__ int bin_of(float v) const { return -whole_steps(steps(v)); }
+    // The weight as a multiple of 2^-S, rounded to a whole number, and its bin. With t = n + f in steps of 1/32 of a power of two,
+    // n from above, 2^(n/32) comes from a table of 32 and a shift, 2^(f/32) = sum (f ln 2 / 32)^k / k! to k = 4 (the first
+    // term left out is 2^-39 of the weight); adding 2^52 rounds, and leaves the whole number in the low bits. The
+    // 64-bit operations are what a pass costs (they run at 32 lanes a clock), so there are seven. No branch, so that the
+    // weights of a chunk overlap.
+    __device__ __forceinline__ u64 mass_of(float v, int& bin) const {
+        const float x = steps(v);
+        const int n = whole_steps(x);
+        bin = -n;
+        const double f = fma(widen(v) - top_wide, scale, -widen(x - kMagicF));
+        double p = fma(kTerm[3], f, kTerm[2]);
+        p = fma(p, f, kTerm[1]);
+        p = fma(p, f, kTerm[0]);
+        p = fma(p, f, 1.0);
+        const double w = s.power[n & 31];
+        const double sum = fma(p, __hiloint2double(__double2hiint(w) + ((n >> 5) + shift << 20), __double2loint(w)), 4503599627370496.0);
+        return n < least_n ? 0 : (u64)__double_as_longlong(sum) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ u64 mass(uint32_t key) const { return fixed(weight(value_of(key))); }
-    __device__ __forceinline__ bool kept(float v, int i) const {
-        const uint32_t k = key_of(v);
-        return v > -INFINITY && (k > cut_key || (k == cut_key && i <= cut_index));
+    __device__ __forceinline__ u64 mass(uint32_t key) const {
+        int unused;
+        return mass_of(value_of(key), unused);
     }
-    // Histogram bin, kBins and more: weight zero. Never rises with v.
-    __device__ __forceinline__ int bin_of(float v) const {
-        const float x = v == top ? 0.f : fminf(top - v, 3.4e38f) * bins;
-        return x < (float)kBins ? (int)x : kBins;
-    }
-
+    __device__ __forceinline__ bool kept(float v, int i) const { return v >= cut_value && (v > cut_value || i <= cut_index); }
     __device__ __forceinline__ static u64 warp_total(u64 v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -390,18 +403,12 @@ template <typename T> struct Row {
         return lane < ranks ? s.slot[parity][lane] : 0;
     }
     __device__ __forceinline__ u64 cluster_sum(u64 v) { return warp_total(exchange(block_sum(v))); }
-    // Three words of rank 0's thread 0 to everyone. Between two calls lies an exchange.
-    __device__ __forceinline__ void tell(u64& a, u64& b, u64& c) {
-        if (rank == 0 && threadIdx.x == 0) {
-            for (int r = 0; r < ranks; ++r) {
-                u64* f = cg::this_cluster().map_shared_rank(s.found, r);
-                f[0] = a; f[1] = b; f[2] = c;
-            }
-        }
+    // A word of rank 0's thread 0 to everyone.
+    __device__ __forceinline__ u64 tell(u64 word) {
+        if (rank == 0 && threadIdx.x == 0)
+            for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s.found[2], r) = word;
         cg::this_cluster().sync();
-        a = s.found[0];
-        b = s.found[1];
-        c = s.found[2];
+        return s.found[2];
     }
 
     __device__ __forceinline__ void put(float v, int i) {
@@ -430,64 +437,85 @@ template <typename T> struct Row {
     // The border of a sum over the kept logits in falling order: count (top-k) or mass (top-p) up to and
     // including the border first reaches the target. Moves the cut there.
     template <bool MASS> __device__ __forceinline__ void cut(int k, float p) {
-        for (int b = threadIdx.x; b < kBins; b += kThreads) s.hist.lo[b] = s.hist.hi[b] = 0;
+        reinterpret_cast<uint4*>(s.hist.lo)[threadIdx.x] = reinterpret_cast<uint4*>(s.hist.hi)[threadIdx.x] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        each([&](float v, int i) {
-            if (!kept(v, i)) return;
-            const int b = bin_of(v);
-            if (b >= kBins) return;
-            if (MASS) {  // 64 bits as two words: the one that overflows the low word carries
-                const u64 w = fixed(weight(v));
-                const uint32_t low = (uint32_t)w, old = atomicAdd(&s.hist.lo[b], low);
-                const uint32_t high = (uint32_t)(w >> 32) + (old + low < old ? 1u : 0u);
-                if (high) atomicAdd(&s.hist.hi[b], high);
-            } else {
-                atomicAdd(&s.hist.lo[b], 1u);
+        each_chunk([&](const Chunk<T>& c, int i0) {
+            if (!(c.most() >= cut_value)) return;
+            int bin[N];
+            u64 w[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (MASS) w[e] = mass_of(c.raw_at(e), bin[e]);
+                else bin[e] = bin_of(c.raw_at(e));
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int b = bin[e];
+                if (-b < least_n || !kept(c.raw_at(e), i0 + e)) continue;
+                if (MASS) {  // 64 bits as two words: the one that overflows the low word carries
+                    const uint32_t low = (uint32_t)w[e], old = atomicAdd(&s.hist.lo[b], low);
+                    const uint32_t high = (uint32_t)(w[e] >> 32) + (old + low < old ? 1u : 0u);
+                    if (high) atomicAdd(&s.hist.hi[b], high);
+                } else {
+                    atomicAdd(&s.hist.lo[b], 1u);
+                }
             }
         });
-        if (threadIdx.x == 0) s.found[0] = ~0ull;
         cg::this_cluster().sync();
-        u64 at = 0, above = 0, target = (u64)k;
-        if (rank == 0) {
-            static_assert(kBins == 4 * kThreads, "a thread's bins are one 16-byte vector");
-            u64 m[4] = {0, 0, 0, 0}, total;
+        // CTA r adds up its share of the bins over all CTAs (one CTA for all of them had 128 KB to fetch); the sums of the
+        // shares say in whose share the border lies
+        const int share = kBins / ranks, per = max(1, share / kThreads), first = (int)threadIdx.x * per;
+        u64 m[kBins / kThreads], sum = 0, total;
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {  // all CTAs' bins under way together
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            m[j] = 0;
+            if (j >= per || first >= share) continue;
+            const int b = rank * share + first + j;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {
                 if (r >= ranks) continue;
-                const uint4 l = reinterpret_cast<const uint4*>(cg::this_cluster().map_shared_rank(s.hist.lo, r))[threadIdx.x];
-                m[0] += l.x; m[1] += l.y; m[2] += l.z; m[3] += l.w;
-                if (MASS) {
-                    const uint4 h = reinterpret_cast<const uint4*>(cg::this_cluster().map_shared_rank(s.hist.hi, r))[threadIdx.x];
-                    m[0] += (u64)h.x << 32; m[1] += (u64)h.y << 32; m[2] += (u64)h.z << 32; m[3] += (u64)h.w << 32;
-                }
+                m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
+                if (MASS) m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
             }
-            u64 before = block_scan(m[0] + m[1] + m[2] + m[3], total);
-            if (MASS) target = target_of(p, total);
-            if (MASS || total > target) {  // else the border lies behind the last logit that weighs anything
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (before < target && before + m[j] >= target) {
-                        s.found[0] = (u64)(threadIdx.x * 4 + j);
-                        s.found[1] = before;
-                    }
-                    before += m[j];
-                }
-            }
-            __syncthreads();
-            at = s.found[0];
-            above = s.found[1];
+            sum += m[j];
         }
-        tell(at, above, target);
-        if (at == ~0ull) return;
-        const int bin = (int)at;
+        u64 before = block_scan(sum, total);
+        const u64 shares = exchange(total);
+        before += warp_total((int)(threadIdx.x & 31) < rank ? shares : 0);
+        total = warp_total(shares);
+        if (!MASS && total <= (u64)k) return;  // the border lies behind the last logit that weighs anything
+        const u64 target = MASS ? target_of(p, total) : (u64)k;
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            if (before < target && before + m[j] >= target) {
+                for (int r = 0; r < ranks; ++r) {
+                    u64* f = cg::this_cluster().map_shared_rank(s.found, r);
+                    f[0] = (u64)(rank * share + first + j);
+                    f[1] = before;
+                }
+            }
+            before += m[j];
+        }
+        cg::this_cluster().sync();
+        const int bin = (int)s.found[0];
+        const u64 above = s.found[1];
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
-        each([&](float v, int i) {
-            if (bin_of(v) == bin && kept(v, i)) put(v, i);
+        // a window around the bin, wider than any rounding, spares most logits the exact question
+        const float width = 1.f / scale_f, slack = 1e-5f * (fabsf(top) + (float)(bin + 2) * width);
+        const bool windowed = top < INFINITY && width < 1e30f && slack < 1e30f;
+        const float from = windowed ? top - ((float)bin + 0.5f) * width - slack : kLowest;
+        const float to = windowed ? top - ((float)bin - 0.5f) * width + slack : INFINITY;
+        each_chunk([&](const Chunk<T>& c, int i0) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float v = c.raw_at(e);
+                if (v >= from && v <= to && bin_of(v) == bin && kept(v, i0 + e)) put(v, i0 + e);
+            }
         });
         const int n = collect();
         if (n <= kCap) {
-            u64 key = 0, unused = 0, unused2 = 0;
+            u64 key = 0;
             if (rank == 0) {
                 if (n <= kPairs) {
                     rank_pairs<MASS>(n, [&](u64 e, int, u64 before, u64 m) {
@@ -496,7 +524,7 @@ template <typename T> struct Row {
                     });
                 } else {
                     const float low = value_of(__reduce_min_sync(0xffffffffu, lowest_key(n)));
-                    const float high = top - (bins > 0.f ? (float)bin / bins : 0.f);
+                    const float high = fminf(to, top_finite);
                     const float per_unit = high - low > 0.f ? (float)(kBins - 1) / fminf(high - low, 3.4e38f) : 0.f;
                     sort_by_bins(s, n, [&](u64 e) {
                         const float d = high - value_of((uint32_t)(e >> 32));
@@ -520,8 +548,8 @@ template <typename T> struct Row {
                 __syncthreads();
                 key = s.found[0];
             }
-            tell(key, unused, unused2);
-            cut_key = (uint32_t)(key >> 32);
+            key = tell(key);
+            cut_value = value_of((uint32_t)(key >> 32));
             cut_index = (int)(0xffffffffu - (uint32_t)key);
             return;
         }
@@ -529,7 +557,7 @@ template <typename T> struct Row {
         auto sum_from = [&](uint32_t from) {  // over the bin's logits with keys >= from
             u64 t = 0;
             each([&](float v, int i) {
-                if (bin_of(v) == bin && key_of(v) >= from && kept(v, i)) t += MASS ? fixed(weight(v)) : 1;
+                if (bin_of(v) == bin && key_of(v) >= from && kept(v, i)) t += MASS ? mass(key_of(v)) : 1;
             });
             return above + cluster_sum(t);
         };
@@ -549,7 +577,7 @@ template <typename T> struct Row {
             });
             if (cluster_sum(t) < ties) index = to;
         }
-        cut_key = key;
+        cut_value = value_of(key);
         cut_index = index + 1;
     }
 
@@ -563,24 +591,38 @@ template <typename T> struct Row {
         const u64 x = t > 0.0 ? (u64)t : 0;  // a NaN draws the first
         return x < total ? x : total - 1;
     }
-    // Smallest weight that stays, in units of 2^-S.
-    __device__ __forceinline__ double least_of(float min_p) const { return min_p > 0.f ? fmin((double)min_p, 1.0) * unit : 0.0; }
+    // The smallest mass that stays: min_p of the largest.
+    __device__ __forceinline__ u64 least_of(float min_p) const {
+        return min_p > 0.f ? (u64)ceil(fmin((double)min_p, 1.0) * (double)mass(key_of(top))) : 0;
+    }
 
     // The draw over everything kept: sums per warp over neighbouring logits, then one warp looks closer.
     __device__ __forceinline__ void draw(float u, float min_p, int64_t* token) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const int per = (nvec + kWarps - 1) / kWarps, from = warp * per, to = min(nvec, from + per);
-        const double least = least_of(min_p);
-        auto of = [&](float v, int i) -> u64 {
-            if (!kept(v, i)) return 0;
-            const double w = weight(v);
-            return w >= least ? fixed(w) : 0;
+        const u64 least = least_of(min_p);
+        // the masses of a chunk's logits that stay; their sum
+        auto masses = [&](int j, u64 (&m)[N]) {
+            const Chunk<T> c = load(j);
+            u64 sum = 0;
+            if (!(c.most() >= cut_value)) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) m[e] = 0;
+                return sum;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                int unused;
+                const u64 w = mass_of(c.raw_at(e), unused);
+                m[e] = kept(c.raw_at(e), base + j * N + e) && w >= least ? w : 0;
+                sum += m[e];
+            }
+            return sum;
         };
         u64 sum = 0;
         for (int j = from + lane; j < to; j += 32) {
-            const Chunk<T> c = load(j);
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum += of(c.at(e), base + j * N + e);
+            u64 m[N];
+            sum += masses(j, m);
         }
         const u64 all = warp_total(sum);
         __syncthreads();
@@ -601,11 +643,7 @@ template <typename T> struct Row {
             const int j = j0 + lane;
 #pragma unroll
             for (int e = 0; e < N; ++e) m[e] = 0;
-            if (j < to) {
-                const Chunk<T> c = load(j);
-#pragma unroll
-                for (int e = 0; e < N; ++e) { m[e] = of(c.at(e), base + j * N + e); own += m[e]; }
-            }
+            if (j < to) own = masses(j, m);
             u64 x = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -650,14 +688,14 @@ template <typename T> struct Row {
 
     // rank 0, with the largest logits in list[0, n): everything that is left to do
     __device__ __forceinline__ void finish_list(int n, int k, float p, float min_p, float u, int64_t* token) {
-        const double least = least_of(min_p);
+        const u64 least = least_of(min_p);
         if (n <= kPairs) {
             u64 key = 0, before = 0, m = 0;
             bool in = false;
             rank_pairs<true>(n, [&](u64 e, int place, u64 b, u64 w) { key = e; before = b; m = w; in = place < k; });
             const u64 total = block_sum(in ? m : 0);  // (its barrier also ends the reading of s.pair)
             if (p < 1.f) in = in && before < target_of(p, total);
-            in = in && weight(value_of((uint32_t)(key >> 32))) >= least;
+            in = in && m >= least;
             if (threadIdx.x < n) s.pair[threadIdx.x] = Entry{key << 32, in ? m : 0};  // falling in ~index: rising in index
             __syncthreads();
             return draw_pairs(n, u, token);
@@ -683,15 +721,13 @@ template <typename T> struct Row {
         return (uint32_t)s.part[threadIdx.x & (kWarps - 1)];
     }
     // The rest over a sorted list of at most PER * kThreads entries, PER neighbours a thread.
-    template <int PER> __device__ __forceinline__ void finish_sorted(int n, float p, double least, float u, int64_t* token) {
+    template <int PER> __device__ __forceinline__ void finish_sorted(int n, float p, u64 least, float u, int64_t* token) {
         u64 m[PER], e[PER], sum = 0, total;
-        double w[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x * PER + j;
             e[j] = i < n ? s.list[i] : 0;
-            w[j] = i < n ? weight(value_of((uint32_t)(e[j] >> 32))) : -1.0;
-            m[j] = i < n ? fixed(w[j]) : 0;
+            m[j] = i < n ? mass((uint32_t)(e[j] >> 32)) : 0;
             sum += m[j];
         }
         u64 before = block_scan(sum, total);
@@ -699,7 +735,7 @@ template <typename T> struct Row {
         int stay = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const bool in = w[j] >= 0.0 && before < target && w[j] >= least;
+            const bool in = e[j] && before < target && m[j] >= least;
             before += m[j];
             if (!in) m[j] = 0;
             stay += in;
@@ -855,7 +891,7 @@ template <typename T> struct Row {
         uint32_t bound = s.picked[0];
         const u64 o = exchange((u64)s.picked[1] << 32 | bound);
         const bool lane_in = (threadIdx.x & 31) < ranks;
-        top = value_of(__reduce_max_sync(0xffffffffu, (uint32_t)(o >> 32)));
+        set_top(value_of(__reduce_max_sync(0xffffffffu, (uint32_t)(o >> 32))));
         bound = max(own, __reduce_min_sync(0xffffffffu, lane_in ? (uint32_t)o : 0xffffffffu));
         if (one) take<false>(c, threadIdx.x, bound_of(bound));
         else if (s.n <= kCap) drop_below(bound);
@@ -878,7 +914,7 @@ template <typename T> struct Row {
         if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = key;
         __syncthreads();
         key = __reduce_max_sync(0xffffffffu, (uint32_t)s.part[threadIdx.x & (kWarps - 1)]);
-        top = value_of(__reduce_max_sync(0xffffffffu, (uint32_t)exchange(key)));
+        set_top(value_of(__reduce_max_sync(0xffffffffu, (uint32_t)exchange(key))));
     }
 
     __device__ __forceinline__ void greedy(int64_t* token) {
@@ -920,12 +956,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     int64_t* token = P.tokens + b;
     const bool greedy = !(temperature > 0.f), by_list = !greedy && k < P.vocab && k <= kListK;
 
-    r.scale = fmax(1.4426950408889634 / (double)temperature, 1e-300);  // at T = inf every finite logit weighs 1
+    const double t = fmax((double)temperature, 1e-20);
+    r.scale = fmax(32.0 * 1.4426950408889634 / t, 1e-300);  // at T = inf every finite logit weighs 1
+    r.scale_f = (float)r.scale;
     r.shift = P.shift;
-    r.unit = (double)(1ull << P.shift);
-    r.bins = (float)((double)kBins / (((double)P.shift + 2.0) * 0.6931471805599453 * (double)temperature));
-    r.cut_key = 0;
-    r.cut_index = 0;
+    r.least_n = -32 * (P.shift + 2);
+    r.cut_value = kLowest;
+    r.cut_index = 0x7fffffff;
+    if (threadIdx.x < 32) shared.power[threadIdx.x] = P.power[threadIdx.x];
     cluster.barrier_wait(std::move(started));
 
     if (by_list) {
@@ -986,6 +1024,7 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int log2v = 0;
     while ((1ll << log2v) < a->vocab) ++log2v;
     P.shift = 62 - log2v < 50 ? 62 - log2v : 50;
+    for (int i = 0; i < 32; ++i) P.power[i] = exp2(i / 32.0);
 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a->batch * C));
