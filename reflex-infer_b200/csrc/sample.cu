@@ -27,6 +27,7 @@
 #include <cooperative_groups.h>
 
 #include <math.h>
+#include <string.h>
 
 #include <type_traits>
 #include <utility>
@@ -42,7 +43,8 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCap = 2048;     // logits that one CTA ranks
-constexpr int kPairs = 128;    // up to here by comparing all pairs, behind by sorting
+constexpr int kPairs = 128;     // a list up to here is ranked by comparing all pairs, a longer one sorted (300: 10 and 4 us)
+constexpr int kPairsCut = 256;  // the same for the bin with a border (200: 4 and 7 us)
 constexpr int kBins = 2048;   // more than 32 * (S + 2), the steps to a weight of zero
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 2 * kThreads;     // groups whose maxima bound the k-th largest logit
@@ -62,7 +64,7 @@ struct SampleParams {
     int32_t top_k0;
     int vocab, slice;  // slice: logits per CTA, a multiple of 8
     int shift;         // S: weights are multiples of 2^-S
-    double power[32];  // 2^(i/32)
+    double power[32];  // 2^(S + i/32), with i * 2^15 taken off the upper word
     int staged;        // general rows keep their slice in shared memory
 };
 
@@ -73,13 +75,15 @@ struct __align__(16) Shared {
     union {
         struct { uint32_t lo[kBins], hi[kBins]; } hist;
         u64 weight[kCap];       // of the sorted list
-        Entry pair[kPairs];     // of the list where all pairs are compared
+        Entry pair[kPairsCut];  // of the list where all pairs are compared
         uint32_t group[kGroups];
     };
     u64 part[kWarps];
+    u64 ends[2][kWarps];
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
+    u64 shares[kMaxCluster][kMaxCluster];  // [CTA][share of the bins]: masses of that CTA's logits
     u64 found[3];              // what one CTA tells all: a bin and the sum before it, a cut
-    double power[32];          // 2^(i/32)
+    double power[32];          // as in SampleParams
     uint32_t picked[3];        // of select(): the bound, the largest key, n before it
     int n;                     // entries that want to be in `list`
 };
@@ -235,7 +239,6 @@ __device__ __forceinline__ void select(Shared& s, float most0, float most1, int 
 
 // (ln 2 / 32)^k / k! for k = 1 .. 4
 __device__ constexpr double kTerm[4] = {0.02166084939249829, 0.00023459619820224677, 1.6938509724371819e-06, 9.172562701824643e-09};
-constexpr float kMagicF = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number
 
 // One CTA's view of its row.
 template <typename T> struct Row {
@@ -247,20 +250,20 @@ template <typename T> struct Row {
     Shared& s;
     int rank, ranks, parity;
     int vocab;
+    int shift;            // S
     bool staged;
     float top;            // the row's largest logit
-    float top_finite;     // the same, at most the largest finite float
-    float scale_f;        // 32 log2(e) / T
-    double top_wide, scale; // 32 log2 of a weight: (v - top) * scale
-    int shift, least_n;   // S; 32 log2 of a weight below which it is 0
+    double top_wide;      // the same, at most the largest finite float
+    double scale;         // 32 log2 of a weight is (v - top_wide) * scale
+    float zero_below;     // logits below weigh less than 2^-S-1: nothing
     float cut_value;      // kept: v > cut_value, or v == cut_value and index <= cut_index
     int cut_index;
 
     __device__ __forceinline__ void set_top(float v) {
         top = v;
-        top_finite = fminf(v, -kLowest);
-        if (v == INFINITY) scale_f = 1e30f;  // next to infinities nothing else weighs
-        top_wide = widen(v);
+        top_wide = (double)fminf(v, -kLowest);
+        zero_below = v == INFINITY ? INFINITY : fmaxf(kLowest, (float)(top_wide - 32.0 * (shift + 2) / scale));
+        cut_value = zero_below;
     }
     // A chunk that reaches over an end of the slice (the first or the last one), element by element.
     __device__ __forceinline__ Chunk<T> load_edge(int j) const {
@@ -318,38 +321,34 @@ template <typename T> struct Row {
             for (int e = 0; e < N; ++e) f(c.at(e), base + j * N + e);
         }
     }
-    // A finite float as a double by moving its bits: the conversion instruction runs at a quarter of the rate of a
-    // multiplication. What is below the smallest normal float becomes zero, an infinity 2^128.
-    __device__ __forceinline__ static double widen(float v) {
-        const uint32_t b = __float_as_uint(v), m = b & 0x7fffffffu;
-        return __hiloint2double(m < 0x00800000u ? 0 : (int)((m >> 3) + 0x38000000u | (b & 0x80000000u)), (int)(b << 29));
-    }
-    // 32 log2 of the weight exp((v - top) / T), rounded to a whole number in fp32: also the histogram's bin, negated.
-    // Never rises as v falls; -4096 for NaN, -inf and all that is far below.
-    __device__ __forceinline__ float steps(float v) const { return fmaxf((fminf(v, -kLowest) - top_finite) * scale_f, -4096.f) + kMagicF; }
-    __device__ __forceinline__ static int whole_steps(float x) { return (int)__float_as_uint(x) - 0x4b400000; }
-    __device__ __forceinline__ int bin_of(float v) const { return -whole_steps(steps(v)); }
-    // The weight as a multiple of 2^-S, rounded to a whole number, and its bin. With t = n + f in steps of 1/32 of a power of two,
-    // n from above, 2^(n/32) comes from a table of 32 and a shift, 2^(f/32) = sum (f ln 2 / 32)^k / k! to k = 4 (the first
-    // term left out is 2^-39 of the weight); adding 2^52 rounds, and leaves the whole number in the low bits. The
-    // 64-bit operations are what a pass costs (they run at 32 lanes a clock), so there are seven. No branch, so that the
-    // weights of a chunk overlap.
+    // The weight exp((v - top) / T) as a multiple of 2^-S, rounded to a whole number, for zero_below <= v <= top; and its
+    // bin, the weight's distance from 1 in steps of 1/32 of a power of two. With 32 log2 of the weight = n + f, n whole and
+    // |f| <= 1/2: 2^(n/32) comes from a table of 32 and a shift, 2^(f/32) = sum (f ln 2 / 32)^k / k! to k = 4 (the first term left out
+    // is 2^-39 of the weight); adding 2^52 rounds, and leaves the whole number in the low bits.
+    // A pass over weights is bound by the integer and compare instructions (half rate) and the nine 64-bit operations. So
+    // n is rounded in 64 bits too, the float is widened by the conversion unit, and the table's entries have their
+    // place in the table taken off the exponent's field: n * 2^15 added to the upper word is the whole shift.
     __device__ __forceinline__ u64 mass_of(float v, int& bin) const {
-        const float x = steps(v);
-        const int n = whole_steps(x);
+        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+        const double d = (double)fminf(v, -kLowest) - top_wide;
+        const double t = fma(d, scale, kMagic);
+        const double f = fma(d, scale, kMagic - t);
+        const int n = __double2loint(t);
         bin = -n;
-        const double f = fma(widen(v) - top_wide, scale, -widen(x - kMagicF));
         double p = fma(kTerm[3], f, kTerm[2]);
         p = fma(p, f, kTerm[1]);
         p = fma(p, f, kTerm[0]);
         p = fma(p, f, 1.0);
         const double w = s.power[n & 31];
-        const double sum = fma(p, __hiloint2double(__double2hiint(w) + ((n >> 5) + shift << 20), __double2loint(w)), 4503599627370496.0);
-        return n < least_n ? 0 : (u64)__double_as_longlong(sum) & 0xfffffffffffffull;
+        const double sum = fma(p, __hiloint2double(__double2hiint(w) + n * 32768, __double2loint(w)), 4503599627370496.0);
+        return (u64)__double_as_longlong(sum) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ int bin_of(float v) const {
+        return -__double2loint(fma((double)fminf(v, -kLowest) - top_wide, scale, 6755399441055744.0));
     }
     __device__ __forceinline__ u64 mass(uint32_t key) const {
         int unused;
-        return mass_of(value_of(key), unused);
+        return value_of(key) >= zero_below ? mass_of(value_of(key), unused) : 0;
     }
     __device__ __forceinline__ bool kept(float v, int i) const { return v >= cut_value && (v > cut_value || i <= cut_index); }
     __device__ __forceinline__ static u64 warp_total(u64 v) {
@@ -451,7 +450,7 @@ template <typename T> struct Row {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int b = bin[e];
-                if (-b < least_n || !kept(c.raw_at(e), i0 + e)) continue;
+                if (!kept(c.raw_at(e), i0 + e)) continue;
                 if (MASS) {  // 64 bits as two words: the one that overflows the low word carries
                     const uint32_t low = (uint32_t)w[e], old = atomicAdd(&s.hist.lo[b], low);
                     const uint32_t high = (uint32_t)(w[e] >> 32) + (old + low < old ? 1u : 0u);
@@ -461,40 +460,65 @@ template <typename T> struct Row {
                 }
             }
         });
-        cg::this_cluster().sync();
-        // CTA r adds up its share of the bins over all CTAs (one CTA for all of them had 128 KB to fetch); the sums of the
-        // shares say in whose share the border lies
-        const int share = kBins / ranks, per = max(1, share / kThreads), first = (int)threadIdx.x * per;
-        u64 m[kBins / kThreads], sum = 0, total;
-#pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            m[j] = 0;
-            if (j >= per || first >= share) continue;
-            const int b = rank * share + first + j;
-#pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) {
-                if (r >= ranks) continue;
-                m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
-                if (MASS) m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
+        // The bins are cut into one share per CTA. Everyone tells everyone what its own logits add to each share, so after one
+        // barrier all know in whose share the border lies, and that CTA alone adds up its share's bins over the cluster.
+        __syncthreads();
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = kBins / ranks;
+        {
+            static_assert(kBins == 4 * kThreads && kWarps >= 2 * kMaxCluster, "a warp's bins lie in one share");
+            const uint4 l = reinterpret_cast<const uint4*>(s.hist.lo)[threadIdx.x];
+            u64 m = (u64)l.x + l.y + l.z + l.w;
+            if (MASS) {
+                const uint4 h = reinterpret_cast<const uint4*>(s.hist.hi)[threadIdx.x];
+                m += (u64)h.x + h.y + h.z + h.w << 32;
             }
-            sum += m[j];
+            m = warp_total(m);
+            if (lane == 0) s.part[warp] = m;
+            __syncthreads();
+            if (threadIdx.x < ranks) {
+                const int per = kWarps / ranks;
+                m = 0;
+                for (int w = 0; w < per; ++w) m += s.part[threadIdx.x * per + w];
+                for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s.shares[rank][threadIdx.x], r) = m;
+            }
         }
-        u64 before = block_scan(sum, total);
-        const u64 shares = exchange(total);
-        before += warp_total((int)(threadIdx.x & 31) < rank ? shares : 0);
-        total = warp_total(shares);
+        cg::this_cluster().sync();
+        u64 in_share = 0;
+        if (lane < ranks)
+            for (int r = 0; r < ranks; ++r) in_share += s.shares[r][lane];
+        u64 total = warp_total(in_share);
         if (!MASS && total <= (u64)k) return;  // the border lies behind the last logit that weighs anything
         const u64 target = MASS ? target_of(p, total) : (u64)k;
+        u64 before = warp_total(lane < rank ? in_share : 0);
+        const u64 mine = __shfl_sync(0xffffffffu, in_share, rank);
+        if (before < target && before + mine >= target) {  // all threads of one CTA
+            const int per = max(1, share / kThreads), first = (int)threadIdx.x * per;
+            u64 m[kBins / kThreads], sum = 0, unused;
 #pragma unroll
-        for (int j = 0; j < kBins / kThreads; ++j) {
-            if (before < target && before + m[j] >= target) {
-                for (int r = 0; r < ranks; ++r) {
-                    u64* f = cg::this_cluster().map_shared_rank(s.found, r);
-                    f[0] = (u64)(rank * share + first + j);
-                    f[1] = before;
+            for (int j = 0; j < kBins / kThreads; ++j) {
+                m[j] = 0;
+                if (j >= per || first >= share) continue;
+                const int b = rank * share + first + j;
+#pragma unroll
+                for (int r = 0; r < kMaxCluster; ++r) {  // all reads under way together
+                    if (r >= ranks) continue;
+                    m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
+                    if (MASS) m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
                 }
+                sum += m[j];
             }
-            before += m[j];
+            before += block_scan(sum, unused);
+#pragma unroll
+            for (int j = 0; j < kBins / kThreads; ++j) {
+                if (before < target && before + m[j] >= target) {
+                    for (int r = 0; r < ranks; ++r) {
+                        u64* f = cg::this_cluster().map_shared_rank(s.found, r);
+                        f[0] = (u64)(rank * share + first + j);
+                        f[1] = before;
+                    }
+                }
+                before += m[j];
+            }
         }
         cg::this_cluster().sync();
         const int bin = (int)s.found[0];
@@ -502,7 +526,7 @@ template <typename T> struct Row {
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
         // a window around the bin, wider than any rounding, spares most logits the exact question
-        const float width = 1.f / scale_f, slack = 1e-5f * (fabsf(top) + (float)(bin + 2) * width);
+        const float width = (float)(1.0 / scale), slack = 1e-5f * (fabsf(top) + (float)(bin + 2) * width);
         const bool windowed = top < INFINITY && width < 1e30f && slack < 1e30f;
         const float from = windowed ? top - ((float)bin + 0.5f) * width - slack : kLowest;
         const float to = windowed ? top - ((float)bin - 0.5f) * width + slack : INFINITY;
@@ -510,43 +534,23 @@ template <typename T> struct Row {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const float v = c.raw_at(e);
-                if (v >= from && v <= to && bin_of(v) == bin && kept(v, i0 + e)) put(v, i0 + e);
+                if (v >= from && v <= to && kept(v, i0 + e) && bin_of(v) == bin) put(v, i0 + e);
             }
         });
         const int n = collect();
         if (n <= kCap) {
             u64 key = 0;
             if (rank == 0) {
-                if (n <= kPairs) {
+                if (n <= kPairsCut) {
                     rank_pairs<MASS>(n, [&](u64 e, int, u64 before, u64 m) {
                         before += above;
                         if (before < target && before + m >= target) s.found[0] = e;
                     });
+                    __syncthreads();
+                    key = s.found[0];
                 } else {
-                    const float low = value_of(__reduce_min_sync(0xffffffffu, lowest_key(n)));
-                    const float high = fminf(to, top_finite);
-                    const float per_unit = high - low > 0.f ? (float)(kBins - 1) / fminf(high - low, 3.4e38f) : 0.f;
-                    sort_by_bins(s, n, [&](u64 e) {
-                        const float d = high - value_of((uint32_t)(e >> 32));
-                        return d > 0.f ? min(kBins - 1, (int)(fminf(d, 3.4e38f) * per_unit)) : 0;
-                    });
-                    constexpr int PER = kCap / kThreads;
-                    u64 m[PER], sum = 0, total;
-#pragma unroll
-                    for (int j = 0; j < PER; ++j) {
-                        const int i = threadIdx.x * PER + j;
-                        m[j] = i < n ? (MASS ? mass((uint32_t)(s.list[i] >> 32)) : 1) : 0;
-                        sum += m[j];
-                    }
-                    u64 before = above + block_scan(sum, total);
-#pragma unroll
-                    for (int j = 0; j < PER; ++j) {
-                        if (before < target && before + m[j] >= target) s.found[0] = s.list[threadIdx.x * PER + j];
-                        before += m[j];
-                    }
+                    key = border<MASS>(n, above, target);
                 }
-                __syncthreads();
-                key = s.found[0];
             }
             key = tell(key);
             cut_value = value_of((uint32_t)(key >> 32));
@@ -557,7 +561,7 @@ template <typename T> struct Row {
         auto sum_from = [&](uint32_t from) {  // over the bin's logits with keys >= from
             u64 t = 0;
             each([&](float v, int i) {
-                if (bin_of(v) == bin && key_of(v) >= from && kept(v, i)) t += MASS ? mass(key_of(v)) : 1;
+                if (kept(v, i) && bin_of(v) == bin && key_of(v) >= from) t += MASS ? mass(key_of(v)) : 1;
             });
             return above + cluster_sum(t);
         };
@@ -664,7 +668,69 @@ template <typename T> struct Row {
         }
     }
 
-    // f(entry, its place, the sum before it, its own mass or 1) for list[0, n), n <= kPairs, all in falling order,
+    // The entry of list[0, n) at which the sum of masses (or 1 each) over falling entries, with `above` before the first, first
+    // reaches the target. A histogram over the ten highest bits in which two entries differ, again and again over the
+    // bin with the border, until one entry is left: two or three rounds of 2 us, however many logits are equal (then their
+    // indexes differ).
+    template <bool MASS> __device__ __forceinline__ u64 border(int n, u64 above, u64 target) {
+        constexpr int PER = kCap / kThreads;
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        u64 e[PER], m[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = threadIdx.x + j * kThreads;
+            e[j] = i < n ? s.list[i] : 0;  // 0: out
+            m[j] = i < n ? (MASS ? mass((uint32_t)(e[j] >> 32)) : 1) : 0;
+        }
+        for (;;) {
+            u64 high = 0, low = ~0ull;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                high = max(high, e[j]);
+                if (e[j]) low = min(low, e[j]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
+                low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+            }
+            __syncthreads();
+            if (lane == 0) { s.ends[0][warp] = high; s.ends[1][warp] = low; }
+            reinterpret_cast<uint2*>(s.hist.lo)[threadIdx.x] = reinterpret_cast<uint2*>(s.hist.hi)[threadIdx.x] = make_uint2(0, 0);
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) { high = max(high, s.ends[0][w]); low = min(low, s.ends[1][w]); }
+            if (high == low) return high;
+            const int first = 63 - __clzll((long long)(high ^ low)), shift = max(0, first - 9);
+            const u64 base = first == 63 ? 0 : high >> (first + 1) << (first + 1);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (!e[j]) continue;
+                const int b = 1023 - (int)((e[j] - base) >> shift);  // the largest in front
+                const uint32_t add = (uint32_t)m[j], old = atomicAdd(&s.hist.lo[b], add);
+                const uint32_t up = (uint32_t)(m[j] >> 32) + (old + add < old ? 1u : 0u);
+                if (up) atomicAdd(&s.hist.hi[b], up);
+            }
+            __syncthreads();
+            const uint2 l = reinterpret_cast<const uint2*>(s.hist.lo)[threadIdx.x], h = reinterpret_cast<const uint2*>(s.hist.hi)[threadIdx.x];
+            const u64 m0 = (u64)h.x << 32 | l.x, m1 = (u64)h.y << 32 | l.y;
+            u64 unused;
+            const u64 before = above + block_scan(m0 + m1, unused);
+            if (before < target && before + m0 + m1 >= target) {
+                const bool second = before + m0 < target;
+                s.found[0] = 2 * threadIdx.x + (second ? 1 : 0);
+                s.found[1] = before + (second ? m0 : 0);
+            }
+            __syncthreads();
+            const int bin = (int)s.found[0];
+            above = s.found[1];
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (e[j] && 1023 - (int)((e[j] - base) >> shift) != bin) e[j] = 0;
+        }
+    }
+
+    // f(entry, its place, the sum before it, its own mass or 1) for list[0, n), n <= kPairsCut, all in falling order,
     // without sorting: a thread compares its entry with every other.
     template <bool MASS, typename F> __device__ __forceinline__ void rank_pairs(int n, F f) {
         const int i = threadIdx.x;
@@ -946,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const T* row = (const T*)P.logits + b * P.row_stride;
     const int lo = min(P.vocab, rank * P.slice), hi = min(P.vocab, lo + P.slice);
     const int phase = (int)(((uintptr_t)(row + lo) & 15) / sizeof(T));
-    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0, P.vocab, false};
+    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0, P.vocab, P.shift, false};
 
     const float temperature = P.temperature ? P.temperature[b] : P.temperature0;
     const float p = P.top_p ? P.top_p[b] : P.top_p0, min_p = P.min_p ? P.min_p[b] : P.min_p0;
@@ -958,10 +1024,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
 
     const double t = fmax((double)temperature, 1e-20);
     r.scale = fmax(32.0 * 1.4426950408889634 / t, 1e-300);  // at T = inf every finite logit weighs 1
-    r.scale_f = (float)r.scale;
-    r.shift = P.shift;
-    r.least_n = -32 * (P.shift + 2);
-    r.cut_value = kLowest;
     r.cut_index = 0x7fffffff;
     if (threadIdx.x < 32) shared.power[threadIdx.x] = P.power[threadIdx.x];
     cluster.barrier_wait(std::move(started));
@@ -1008,11 +1070,12 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
 
-    // CTAs of a row: one where the rows fill the GPU, else as many as fill it while a CTA keeps 8 logits or more a thread,
-    // and more for a slice that then stays in shared memory.
+    // CTAs of a row: one where the rows alone give every SM one (256 x 131072 fp32: 41.7 us, with two a row 57.6), else as many as
+    // give every SM two while a CTA keeps 8 logits or more a thread (64 x 131072 bf16: eight 46.9 us, four 52.2: rows
+    // differ in work by their settings, and finer pieces even that out).
     int C = 1;
     auto slice_of = [&](int c) { return round_up<int64_t>(ceil_div<int64_t>(a->vocab, c), 8); };
-    while (C < kMaxCluster && a->batch * C < sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
+    while (C < kMaxCluster && a->batch < sm_count() && a->batch * C < 2 * sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
     const int64_t slice = slice_of(C);
     const size_t bytes = round_up<size_t>((size_t)(slice + 8) * e, 16);
     const bool staged = bytes <= (a->batch * C > sm_count() ? kStageTwo : kStageMax);
@@ -1024,7 +1087,13 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int log2v = 0;
     while ((1ll << log2v) < a->vocab) ++log2v;
     P.shift = 62 - log2v < 50 ? 62 - log2v : 50;
-    for (int i = 0; i < 32; ++i) P.power[i] = exp2(i / 32.0);
+    for (int i = 0; i < 32; ++i) {
+        const double w = ldexp(exp2(i / 32.0), P.shift);
+        uint64_t bits;
+        memcpy(&bits, &w, 8);
+        bits -= (uint64_t)i << 47;
+        memcpy(&P.power[i], &bits, 8);
+    }
 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a->batch * C));
