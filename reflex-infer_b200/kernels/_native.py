@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 from typing import Optional
 
@@ -331,6 +332,22 @@ def stream_handle(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def stream_of(index: int) -> int:
+    """The current stream of device ``index``, without the ``torch.cuda.Stream`` object around it."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def same_device(name: str, first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The index of the CUDA device that all tensors are on; ``require_cuda``'s errors otherwise."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        require_cuda(name, first, *others)
+    return index
+
+
 def check(status: int) -> None:
     if status == RFX_SUCCESS:
         return
@@ -350,6 +367,35 @@ def call(name: str, args: C.Structure, dev: torch.device) -> None:
         return
     with torch.cuda.device(dev):
         check(fn(C.byref(args)))
+
+
+class Entry:
+    """An ``int f(const Args*)`` entry point whose struct is packed in one go: ``entry(device_index, *fields)``
+    with every field of the mirror in its order, pointers as integers (0: NULL). A ctypes structure takes
+    several times as long to fill, which for a small launch is longer than the kernel runs."""
+
+    _CODES = {vp: "P", i64: "q", C.c_int: "i", C.c_float: "f", C.c_double: "d", C.c_size_t: "N"}
+
+    def __init__(self, name: str, mirror):
+        layout = struct.Struct("@" + "".join(self._CODES.get(t, "P") for _, t in mirror._fields_) + "0q")
+        assert layout.size == C.sizeof(mirror), mirror.__name__
+        self._name, self._pack, self._fn = name, layout.pack, None
+
+    def _bind(self):
+        self._fn = lib()[self._name]  # a function object of its own: the bytes go in place of the struct's pointer
+        self._fn.restype, self._fn.argtypes = C.c_int, [C.c_char_p]
+        return self._fn
+
+    def __call__(self, index: int, *fields) -> None:
+        fn = self._fn or self._bind()
+        data = self._pack(*fields)
+        if index == torch.cuda.current_device():
+            status = fn(data)
+        else:
+            with torch.cuda.device(index):
+                status = fn(data)
+        if status:
+            check(status)
 
 
 def peer_export(device_ptr: int, dev: torch.device) -> bytes:

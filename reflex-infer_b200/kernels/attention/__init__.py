@@ -30,7 +30,7 @@ from typing import Optional
 import torch
 
 from .. import _native as N
-from ..rope import _norm_args
+from ..rope import _norm_inputs
 
 
 def _resolve_head_repeat(num_heads_q: int, num_heads_kv: int) -> int:
@@ -474,6 +474,9 @@ def rope_append(
                           interleaved=interleaved, k_scales=k_scales, v_scales=v_scales).run()
 
 
+_norm_append = N.Entry("rfx_qk_norm_rope_append", N.QkNormRopeArgs)
+
+
 def qk_norm_rope_append(
     q: Optional[torch.Tensor],
     k_new: torch.Tensor,
@@ -504,27 +507,32 @@ def qk_norm_rope_append(
     is; its row of ``q_out`` is zero, or unchanged if ``q_out`` is ``q``.
     """
     name = "qk_norm_rope_append"
-    dev = N.require_cuda(name, q, k_new, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin, q_weight,
-                         k_weight, q_out, k_scales, v_scales)
+    if positions is None:
+        raise ValueError(f"{name}: positions are required")
+    index = N.same_device(name, k_new, q, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin, q_weight,
+                          k_weight, q_out, k_scales, v_scales)
     if k_new.stride(-1) != 1:
         k_new = k_new.contiguous()
     if v_new.stride(-1) != 1:
         v_new = v_new.contiguous()
     if q is not None and q.stride(-1) != 1:
         q = q.contiguous()
-    if positions is None:
-        raise ValueError(f"{name}: positions are required")
-    a, keep = _norm_args(name, q, k_new, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    n, hkv, D = k_new.shape
-    if v_new.shape != k_new.shape or v_new.dtype != k_new.dtype:
-        raise ValueError(f"{name}: v_new must be like k_new, {tuple(k_new.shape)} in {k_new.dtype}")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride():
+    cos, sin, positions, q_weight, k_weight = _norm_inputs(name, q, k_new, q_weight, k_weight, cos, sin, positions, eps)
+    code = N.dtype_code(k_new)
+    shape, dtype, pool, strides = k_new.shape, k_new.dtype, k_cache.shape, k_cache.stride()
+    n, hkv, D = shape
+    if v_new.shape != shape or v_new.dtype != dtype:
+        raise ValueError(f"{name}: v_new must be like k_new, {tuple(shape)} in {dtype}")
+    if len(pool) != 4 or v_cache.shape != pool or v_cache.stride() != strides:
         raise ValueError(f"{name}: caches must both be [num_blocks, H_kv, block_size, D] with one stride pattern")
-    nb, ch, bs, cd = k_cache.shape
-    if (hkv, D) != (ch, cd):
+    nb, ch, bs, cd = pool
+    if hkv != ch or D != cd:
         raise ValueError(f"{name}: input heads/head_dim {(hkv, D)} do not match the cache {(ch, cd)}")
-    kv_int8 = k_cache.dtype == torch.int8
-    if kv_int8:
+    if strides[3] != 1:
+        raise ValueError(f"{name}: the head_dim axis of the caches must be contiguous")
+    kv_int8 = 0
+    if k_cache.dtype == torch.int8:
+        kv_int8 = 1
         if v_cache.dtype != torch.int8 or k_scales is None or v_scales is None:
             raise ValueError(f"{name}: an int8 pool needs int8 k_cache and v_cache and k_scales, v_scales")
         if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
@@ -532,34 +540,36 @@ def qk_norm_rope_append(
         for t in (k_scales, v_scales):
             if t.dtype != torch.float32 or tuple(t.shape) != (nb, ch, bs) or not t.is_contiguous():
                 raise ValueError(f"{name}: scales must be contiguous float32 [{nb}, {ch}, {bs}]")
-        a.kv_int8, a.k_scales, a.v_scales = 1, k_scales.data_ptr(), v_scales.data_ptr()
-    elif k_cache.dtype != k_new.dtype or v_cache.dtype != k_new.dtype:
-        raise RuntimeError(f"{name}: input dtype {k_new.dtype} does not match cache dtype {k_cache.dtype}")
-    if k_cache.stride(3) != 1:
-        raise ValueError(f"{name}: the head_dim axis of the caches must be contiguous")
-    if slot_mapping.shape != (n,):
+    elif k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise RuntimeError(f"{name}: input dtype {dtype} does not match cache dtype {k_cache.dtype}")
+    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != n:
         raise ValueError(f"{name}: slot_mapping must be [N]={n}, got {tuple(slot_mapping.shape)}")
     if slot_mapping.dtype != torch.int64:
         slot_mapping = slot_mapping.to(torch.int64)
     slot_mapping = slot_mapping.contiguous()
+    hq = q_sn = q_sh = qo_sn = qo_sh = 0
     if q is None:
         q_out = None
     else:
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(-1) != 1:
             raise ValueError(f"{name}: q_out must be shaped like q, in its dtype, with a contiguous last axis")
         elif any(st == 0 and size > 1 for st, size in zip(q_out.stride(), q_out.shape)):
             raise ValueError(f"{name}: q_out must not be an expanded view")
-        a.q_out = q_out.data_ptr()
-        a.q_out_stride_n, a.q_out_stride_h, _ = q_out.stride()
-    a.v, a.k_cache, a.v_cache, a.slot_mapping = (v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                                 slot_mapping.data_ptr())
-    a.v_stride_n, a.v_stride_h, _ = v_new.stride()
-    a.num_blocks, a.block_size = nb, bs
-    a.cache_stride_blk, a.cache_stride_h, a.cache_stride_pos, _ = k_cache.stride()
-    a.stream = N.stream_handle(dev)
-    N.call("rfx_qk_norm_rope_append", a, dev)
+        hq = q.shape[1]
+        q_sn, q_sh, _ = q.stride()
+        qo_sn, qo_sh, _ = q_out.stride()
+    k_sn, k_sh, _ = k_new.stride()
+    v_sn, v_sh, _ = v_new.stride()
+    _norm_append(index,
+                 q.data_ptr() if hq else 0, k_new.data_ptr(), v_new.data_ptr(), q_out.data_ptr() if hq else 0, 0,
+                 k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), cos.data_ptr(),
+                 sin.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+                 n, hq, hkv, D, nb, bs, cos.shape[0],
+                 q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, qo_sn, qo_sh, 0, 0, strides[0], strides[1], strides[2], cos.stride(0),
+                 eps, 1 if interleaved else 0, 1 if cos.dtype == torch.float32 else 0, code, kv_int8,
+                 k_scales.data_ptr() if kv_int8 else 0, v_scales.data_ptr() if kv_int8 else 0, N.stream_of(index))
     return q_out
 
 

@@ -155,6 +155,12 @@ class PageMoves(NamedTuple):
     count: Optional[torch.Tensor] = None
 
 
+_fork = N.Entry("rfx_kv_fork", N.KvForkArgs)
+_free = N.Entry("rfx_kv_free", N.KvFreeArgs)
+_compact = N.Entry("rfx_kv_compact", N.KvCompactArgs)
+_copy = N.Entry("rfx_kv_copy_pages", N.KvCopyArgs)
+
+
 def _check_table(name, block_table, ref_counts):
     if block_table.dim() != 2 or block_table.dtype != torch.int64:
         raise ValueError(f"{name}: block_table must be int64 [rows, max_blocks], "
@@ -173,10 +179,10 @@ def _check_table(name, block_table, ref_counts):
 def _int32_vector(name, what, t, n=None):
     if t.dim() != 1 or (n is not None and t.shape[0] != n):
         raise ValueError(f"{name}: {what} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
-    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        raise ValueError(f"{name}: {what} must hold whole numbers, got {t.dtype}")
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+            raise ValueError(f"{name}: {what} must hold whole numbers, got {t.dtype}")
+        t = t.clamp(-1, 2**31 - 1).to(torch.int32) if t.dtype == torch.int64 else t.to(torch.int32)
     return t.contiguous()
 
 
@@ -201,7 +207,7 @@ def kv_fork(
     """
     N.check_backend(backend)
     name = "kv_fork"
-    dev = N.require_cuda(name, block_table, context_lens, parents, ref_counts)
+    index = N.same_device(name, block_table, context_lens, parents, ref_counts)
     _check_table(name, block_table, ref_counts)
     if int(block_size) <= 0:
         raise ValueError(f"{name}: block_size must be positive, got {block_size}")
@@ -209,17 +215,12 @@ def kv_fork(
     context_lens = _int32_vector(name, "context_lens", context_lens, batch)
     parents = _int32_vector(name, "parents", parents)
     n = parents.shape[0]
-    child = torch.empty((n, max_blocks), dtype=torch.int64, device=dev)
-    pages = torch.empty((2, n), dtype=torch.int64, device=dev)
-    rows = torch.empty(n, dtype=torch.int32, device=dev)
-    src, dst = pages[0], pages[1]
-    a = N.KvForkArgs(
-        block_table=N.ptr(block_table), context_lens=N.ptr(context_lens), parents=N.ptr(parents),
-        ref_counts=N.ptr(ref_counts), child_table=N.ptr(child), src_pages=N.ptr(src), dst_pages=N.ptr(dst),
-        copy_rows=N.ptr(rows), n_children=n, batch=batch, max_blocks=max_blocks, bt_stride_b=block_table.stride(0),
-        num_blocks=ref_counts.shape[0], block_size=int(block_size), stream=N.stream_handle(dev),
-    )
-    N.call("rfx_kv_fork", a, dev)
+    child = block_table.new_empty((n, max_blocks))
+    src, dst = block_table.new_empty((2, n))
+    rows = parents.new_empty(n)
+    _fork(index, block_table.data_ptr(), context_lens.data_ptr(), parents.data_ptr(), ref_counts.data_ptr(),
+          child.data_ptr(), src.data_ptr(), dst.data_ptr(), rows.data_ptr(),
+          n, batch, max_blocks, block_table.stride(0), ref_counts.shape[0], int(block_size), N.stream_of(index))
     return child, PageMoves(src, dst, rows)
 
 
@@ -235,15 +236,11 @@ def kv_free(
     its pages up once; a row outside the table is skipped."""
     N.check_backend(backend)
     name = "kv_free"
-    dev = N.require_cuda(name, block_table, rows, ref_counts)
+    index = N.same_device(name, block_table, rows, ref_counts)
     _check_table(name, block_table, ref_counts)
     rows = _int32_vector(name, "rows", rows)
-    a = N.KvFreeArgs(
-        block_table=N.ptr(block_table), rows=N.ptr(rows), ref_counts=N.ptr(ref_counts), n_rows=rows.shape[0],
-        batch=block_table.shape[0], max_blocks=block_table.shape[1], bt_stride_b=block_table.stride(0),
-        num_blocks=ref_counts.shape[0], stream=N.stream_handle(dev),
-    )
-    N.call("rfx_kv_free", a, dev)
+    _free(index, block_table.data_ptr(), rows.data_ptr(), ref_counts.data_ptr(), rows.shape[0], block_table.shape[0],
+          block_table.shape[1], block_table.stride(0), ref_counts.shape[0], N.stream_of(index))
 
 
 def kv_compact(
@@ -262,22 +259,17 @@ def kv_compact(
     """
     N.check_backend(backend)
     name = "kv_compact"
-    dev = N.require_cuda(name, block_table, ref_counts)
+    index = N.same_device(name, block_table, ref_counts)
     _check_table(name, block_table, ref_counts)
     num = ref_counts.shape[0]
-    page_map = torch.empty(num, dtype=torch.int64, device=dev)
-    pages = torch.empty((2, num // 2 + 1), dtype=torch.int64, device=dev)
+    page_map = block_table.new_empty(num)
+    src, dst = block_table.new_empty((2, num // 2 + 1))
     need = int(N.lib().rfx_kv_compact_workspace_bytes(num))
-    # the number of moves stands in front of the scratch
-    words = torch.empty(64 + need // 4, dtype=torch.int32, device=dev)
-    src, dst, count = pages[0], pages[1], words[:1]
-    a = N.KvCompactArgs(
-        block_table=N.ptr(block_table), ref_counts=N.ptr(ref_counts), page_map=N.ptr(page_map), src_pages=N.ptr(src),
-        dst_pages=N.ptr(dst), n_moves=N.ptr(count), batch=block_table.shape[0], max_blocks=block_table.shape[1],
-        bt_stride_b=block_table.stride(0), num_blocks=num, workspace=words.data_ptr() + 256, workspace_bytes=need,
-        stream=N.stream_handle(dev),
-    )
-    N.call("rfx_kv_compact", a, dev)
+    words = ref_counts.new_empty(64 + need // 4)  # the number of moves stands in front of the scratch
+    count = words[:1]
+    _compact(index, block_table.data_ptr(), ref_counts.data_ptr(), page_map.data_ptr(), src.data_ptr(), dst.data_ptr(),
+             count.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0), num,
+             words.data_ptr() + 256, need, N.stream_of(index))
     return page_map, PageMoves(src, dst, None, count)
 
 
@@ -307,12 +299,12 @@ def kv_copy_pages(
     if len(ks) != len(vs) or not ks:
         raise ValueError(f"{name}: as many k as v caches are needed, at least one; got {len(ks)} and {len(vs)}")
     src, dst, rows, count = moves
-    dev = N.require_cuda(name, *ks, *vs, src, dst, rows, count)
     first = ks[0]
+    index = N.same_device(name, first, src, dst, rows, count, *ks, *vs)
     _check_pool(name, first, vs[0])
     shape, strides, dtype = first.shape, first.stride(), first.dtype
     for t in ks + vs:
-        if t.shape != shape or t.stride() != strides or t.dtype != dtype:
+        if t is not first and (t.shape != shape or t.stride() != strides or t.dtype != dtype):
             raise ValueError(f"{name}: the caches of all layers must share one shape, stride pattern and dtype")
     if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.dim() != 1 or dst.shape != src.shape:
         raise ValueError(f"{name}: moves.src and moves.dst must be int64 [n]")
@@ -322,28 +314,27 @@ def kv_copy_pages(
         rows = _int32_vector(name, "moves.rows", rows, n)
     if count is not None and (count.dtype != torch.int32 or count.numel() != 1):
         raise ValueError(f"{name}: moves.count must be one int32")
-    int8 = dtype == torch.int8
     L = len(ks)
     array = N.vp * L
-    a = N.KvCopyArgs(
-        k_caches=array(*[t.data_ptr() for t in ks]), v_caches=array(*[t.data_ptr() for t in vs]),
-        src_pages=N.ptr(src), dst_pages=N.ptr(dst), copy_rows=N.ptr(rows), n_moves=N.ptr(count),
-        n_layers=L, n_pairs=n, num_kv_heads=shape[1], head_dim=shape[3], num_blocks=shape[0], block_size=shape[2],
-        cache_stride_blk=strides[0], cache_stride_h=strides[1], cache_stride_pos=strides[2],
-        dtype=0 if int8 else N.dtype_code(first), kv_int8=int(int8), stream=N.stream_handle(dev),
-    )
-    if int8:
+    k_ptrs, v_ptrs = array(*[t.data_ptr() for t in ks]), array(*[t.data_ptr() for t in vs])
+    int8, k_scale_ptrs, v_scale_ptrs = 0, None, None
+    if dtype == torch.int8:
+        int8 = 1
         if k_scales is None or v_scales is None:
             raise ValueError(f"{name}: an int8 pool needs k_scales and v_scales")
         sk, sv = _layers(k_scales), _layers(v_scales)
-        N.require_cuda(name, first, *sk, *sv)
+        N.same_device(name, first, *sk, *sv)
         if len(sk) != L or len(sv) != L:
             raise ValueError(f"{name}: every layer needs its scales")
         for t in sk + sv:
             if t.dtype != torch.float32 or t.shape != shape[:3] or not t.is_contiguous():
                 raise ValueError(f"{name}: scales must be contiguous float32 {list(shape[:3])}")
-        a.k_scales, a.v_scales = array(*[t.data_ptr() for t in sk]), array(*[t.data_ptr() for t in sv])
-    N.call("rfx_kv_copy_pages", a, dev)
+        k_scale_ptrs, v_scale_ptrs = array(*[t.data_ptr() for t in sk]), array(*[t.data_ptr() for t in sv])
+    _copy(index, C.addressof(k_ptrs), C.addressof(v_ptrs), C.addressof(k_scale_ptrs) if int8 else 0,
+          C.addressof(v_scale_ptrs) if int8 else 0, src.data_ptr(), dst.data_ptr(),
+          0 if rows is None else rows.data_ptr(), 0 if count is None else count.data_ptr(),
+          L, n, shape[1], shape[3], shape[0], shape[2], strides[0], strides[1], strides[2],
+          0 if int8 else N.dtype_code(first), int8, N.stream_of(index))
 
 
 # The reference's surface; the page bookkeeping above is an addition, imported by name.

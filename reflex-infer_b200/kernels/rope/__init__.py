@@ -151,67 +151,68 @@ def build_rope_tables(
     return cos, sin
 
 
-def _norm_args(name, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    """The checks and fields that the dense form and the append share. Returns the args struct, the
-    device and the tensors that have to outlive the call. ``q`` may be ``None`` (no query heads)."""
-    if k.dim() != 3 or (q is not None and (q.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2])):
+_dense = N.Entry("rfx_qk_norm_rope", N.QkNormRopeArgs)
+
+
+def _norm_inputs(name, q, k, q_weight, k_weight, cos, sin, positions, eps):
+    """The checks that the dense form and the append share; returns ``(cos, sin, positions, q_weight, k_weight)``
+    as the kernel takes them. ``q`` may be ``None`` (no query heads)."""
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or (q is not None and (q.dim() != 3 or q.shape[0] != shape[0] or q.shape[2] != shape[2])):
         raise ValueError(f"{name}: q must be [N, H_q, D] and k [N, H_kv, D]; "
-                         f"got {None if q is None else tuple(q.shape)} and {tuple(k.shape)}")
-    n, hkv, D = k.shape
+                         f"got {None if q is None else tuple(q.shape)} and {tuple(shape)}")
+    n, _, D = shape
     if D % 2 != 0:
         raise ValueError("head_dim must be even for RoPE")
-    dtype = k.dtype
-    code = N.dtype_code(k)
     if q is not None and q.dtype != dtype:
         raise RuntimeError(f"{name}: q dtype {q.dtype} differs from k dtype {dtype}")
     for w in (q_weight, k_weight):
-        if w.shape != (D,):
+        if w.dim() != 1 or w.shape[0] != D:
             raise ValueError(f"{name}: weights must be [{D}], got {tuple(w.shape)}")
         if w.dtype != dtype:
             raise RuntimeError(f"{name}: weight dtype {w.dtype} differs from the activations' {dtype}")
     if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape:
         raise ValueError(f"{name}: cos/sin must both be [rows, {D}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
-    if cos.dtype != sin.dtype or cos.dtype not in (dtype, torch.float32):
+    table = cos.dtype
+    if (table != torch.float32 and table != dtype) or sin.dtype != table:
         cos, sin = cos.to(dtype), sin.to(dtype)
-    if cos.stride(1) != 1 or sin.stride() != cos.stride():
+    if not (cos.is_contiguous() and sin.is_contiguous()) and (cos.stride(1) != 1 or sin.stride() != cos.stride()):
         cos, sin = cos.contiguous(), sin.contiguous()
     if positions is not None:
-        if positions.shape != (n,):
+        if positions.dim() != 1 or positions.shape[0] != n:
             raise ValueError(f"{name}: positions must be [N]={n}, got {tuple(positions.shape)}")
         if positions.dtype != torch.int32:
+            if positions.dtype == torch.int64:
+                positions = positions.clamp(-1, 2**31 - 1)
             positions = positions.to(torch.int32)
         positions = positions.contiguous()
     elif n > cos.shape[0]:
         raise ValueError(f"{name}: {n} tokens without positions need as many table rows, got {cos.shape[0]}")
-    eps = float(eps)
-    if not eps >= 0.0:
+    if not 0.0 <= eps < 3e38:
         raise ValueError(f"{name}: eps must not be negative, got {eps}")
-    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
-    a = N.QkNormRopeArgs()
-    a.k, a.cos, a.sin = k.data_ptr(), cos.data_ptr(), sin.data_ptr()
-    a.q_weight, a.k_weight, a.positions = q_weight.data_ptr(), k_weight.data_ptr(), N.ptr(positions)
-    a.n_tokens, a.num_kv_heads, a.head_dim = n, hkv, D
-    a.k_stride_n, a.k_stride_h, _ = k.stride()
-    if q is not None:
-        a.q, a.num_q_heads = q.data_ptr(), q.shape[1]
-        a.q_stride_n, a.q_stride_h, _ = q.stride()
-    a.table_rows, a.table_stride = cos.shape[0], cos.stride(0)
-    a.eps, a.interleaved = eps, int(bool(interleaved))
-    a.tables_f32, a.dtype = int(cos.dtype == torch.float32), code
-    return a, (cos, sin, positions, q_weight, k_weight)
+    return cos, sin, positions, q_weight.contiguous(), k_weight.contiguous()
 
 
-def _norm_rope(name, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-    dev = N.require_cuda(name, q, k, q_weight, k_weight, cos, sin, positions)
-    a, keep = _norm_args(name, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
-    a.q_out_stride_n, a.q_out_stride_h, _ = q_out.stride()
-    a.k_out_stride_n, a.k_out_stride_h, _ = k_out.stride()
-    a.stream = N.stream_handle(dev)
-    N.call("rfx_qk_norm_rope", a, dev)
+def _norm_rope(name, q, k, in_place, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+    index = N.same_device(name, k, q, q_weight, k_weight, cos, sin, positions)
+    cos, sin, positions, q_weight, k_weight = _norm_inputs(name, q, k, q_weight, k_weight, cos, sin, positions, eps)
+    code = N.dtype_code(k)
+    if in_place:
+        q_out, k_out = q, k
+    else:
+        q_out, k_out = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
+    n, hkv, D = k.shape
+    q_sn, q_sh, _ = q.stride()
+    k_sn, k_sh, _ = k.stride()
+    qo_sn, qo_sh, _ = q_out.stride()
+    ko_sn, ko_sh, _ = k_out.stride()
+    _dense(index,
+           q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0,
+           0, 0 if positions is None else positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+           q_weight.data_ptr(), k_weight.data_ptr(),
+           n, q.shape[1], hkv, D, 0, 0, cos.shape[0],
+           q_sn, q_sh, k_sn, k_sh, 0, 0, qo_sn, qo_sh, ko_sn, ko_sh, 0, 0, 0, cos.stride(0),
+           eps, 1 if interleaved else 0, 1 if cos.dtype == torch.float32 else 0, code, 0, 0, 0, N.stream_of(index))
     return q_out, k_out
 
 
@@ -243,7 +244,7 @@ def qk_norm_rope(
         q = q.contiguous()
     if k.stride(-1) != 1:
         k = k.contiguous()
-    return _norm_rope("qk_norm_rope", q, k, None, None, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _norm_rope("qk_norm_rope", q, k, False, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 def qk_norm_rope_(
@@ -268,7 +269,7 @@ def qk_norm_rope_(
             raise ValueError("qk_norm_rope_: the head_dim axis must be contiguous to work in place")
         if any(st == 0 and size > 1 for st, size in zip(t.stride(), t.shape)):
             raise ValueError("qk_norm_rope_: an expanded view has no rows of its own to work in place")
-    return _norm_rope("qk_norm_rope_", q, k, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    return _norm_rope("qk_norm_rope_", q, k, True, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 # The reference's surface; qk_norm_rope and qk_norm_rope_ are additions, imported by name.

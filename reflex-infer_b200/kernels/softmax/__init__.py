@@ -42,12 +42,19 @@ def online_softmax(
     return y.reshape(x.shape)
 
 
+_INF = float("inf")
+_MOST = torch.finfo(torch.float32).max
+_sample = N.Entry("rfx_sample_tokens", N.SampleArgs)
+
+
 def _setting(name, what, value, B, dtype, low, high):
     """``(tensor or None, number)`` of a sampling setting; only numbers are checked against their range."""
     if isinstance(value, torch.Tensor):
         if value.shape != (B,):
             raise ValueError(f"{name}: {what} must be a number or [{B}], got {tuple(value.shape)}")
         if value.dtype != dtype:
+            if dtype == torch.int32 and value.dtype == torch.int64:
+                value = value.clamp(-1, 2**31 - 1)
             value = value.to(dtype)
         return value.contiguous(), 0
     if not low <= value <= high:
@@ -85,28 +92,25 @@ def sample_tokens(
     B, vocab = logits.shape
     if uniform.shape != (B,):
         raise ValueError(f"{name}: uniform must be [{B}], got {tuple(uniform.shape)}")
-    inf = float("inf")
-    temperature, temperature_all = _setting(name, "temperature", temperature, B, torch.float32, 0.0, inf)
-    top_k, top_k_all = _setting(name, "top_k", top_k, B, torch.int32, 0, inf)
+    temperature, temperature_all = _setting(name, "temperature", temperature, B, torch.float32, 0.0, _INF)
+    top_k, top_k_all = _setting(name, "top_k", top_k, B, torch.int32, 0, _INF)
     top_p, top_p_all = _setting(name, "top_p", top_p, B, torch.float32, 0.0, 1.0)
     min_p, min_p_all = _setting(name, "min_p", min_p, B, torch.float32, 0.0, 1.0)
-    dev = N.require_cuda(name, logits, uniform, temperature, top_k, top_p, min_p, out)
-    if logits.stride(1) != 1 and vocab > 1:
+    index = N.same_device(name, logits, uniform, temperature, top_k, top_p, min_p, out)
+    if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     if uniform.dtype != torch.float32:
         uniform = uniform.to(torch.float32)
     uniform = uniform.contiguous()
     if out is None:
-        out = torch.empty(B, dtype=torch.int64, device=dev)
+        out = logits.new_empty(B, dtype=torch.int64)
     elif out.shape != (B,) or out.dtype != torch.int64 or not out.is_contiguous():
         raise ValueError(f"{name}: out must be contiguous int64 [{B}]")
-    a = N.SampleArgs(
-        logits=logits.data_ptr(), uniform=uniform.data_ptr(), temperature=N.ptr(temperature), top_k=N.ptr(top_k),
-        top_p=N.ptr(top_p), min_p=N.ptr(min_p), tokens=out.data_ptr(), batch=B, vocab=vocab, row_stride=logits.stride(0),
-        temperature_all=temperature_all, top_k_all=int(min(top_k_all, vocab)), top_p_all=top_p_all, min_p_all=min_p_all,
-        dtype=N.dtype_code(logits), stream=N.stream_handle(dev),
-    )
-    N.call("rfx_sample_tokens", a, dev)
+    _sample(index, logits.data_ptr(), uniform.data_ptr(), 0 if temperature is None else temperature.data_ptr(),
+            0 if top_k is None else top_k.data_ptr(), 0 if top_p is None else top_p.data_ptr(),
+            0 if min_p is None else min_p.data_ptr(), out.data_ptr(), B, vocab, logits.stride(0),
+            _INF if temperature_all > _MOST else temperature_all, int(min(top_k_all, vocab)), top_p_all, min_p_all, N.dtype_code(logits),
+            N.stream_of(index))
     return out
 
 
