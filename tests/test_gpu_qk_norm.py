@@ -2,10 +2,10 @@
 formula in 64 bits.
 
 Tolerance, derived before the first run: with u = 2^-24 the fp32 sum of D squares is off by at most D*u of
-its value, so the factor 1/sqrt is off by D*u/2 and a few roundings (inv_d, the sum with eps, sqrt, divide:
-5u); the two products of an output carry 3 more roundings each and their sum one: every output is within
-(D/2 + 9) * u * (|n_i c| + |n_j s|) of the formula before it is rounded once to the type (half a step,
-eps / 2, relative; half the smallest subnormal below the normal range)."""
+its value, so the factor 1/sqrt is off by D*u/2 and 5u of roundings (inv_d and the sum with eps, halved by the
+root; the reciprocal root's 2 ulp); an output's weight times table factor, product, sum and product with 1/sqrt
+add 4u: every output is within (D/2 + 9) * u * (|n_i c| + |n_j s|) of the formula before it is rounded once to
+the type (half a step, eps / 2, relative; half the smallest subnormal below the normal range)."""
 from __future__ import annotations
 
 import pytest
