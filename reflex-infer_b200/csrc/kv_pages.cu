@@ -7,6 +7,8 @@
 // takes the caches of all of them in one launch.
 //
 // Algorithmic bytes: 4 per page (counts) and 8 per table entry read and written; copies 2 * moved bytes.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
 #include "ptx.cuh"
 
@@ -95,16 +97,17 @@ __device__ __forceinline__ Child child_of(const ForkParams& P, int64_t i) {
 }
 
 // One CTA hands out the pages: children in order, 1024 at a time, each group's pages from one walk over the
-// counts, 32 pages a thread, that stops where the last one was found and goes on there for the next group.
-constexpr int kForkThreads = 1024, kForkPages = 32;
-__global__ void __launch_bounds__(kForkThreads) kv_fork_take_kernel(const ForkParams P) {
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
+// counts that stops where the last one was found and goes on there for the next group: first four pages a thread, as
+// free pages are often near, then 32.
+constexpr int kForkThreads = 1024, kForkPages = 32, kForkFirst = 4;
+__device__ __forceinline__ void fork_take(const ForkParams& P) {
     __shared__ int part[32];
     __shared__ int fresh[kForkThreads];
     __shared__ int64_t next_from;
     const bool aligned = ((uintptr_t)P.counts & 15) == 0;
     int64_t from = 0;
+    // the first pages' counts are on their way while the children's lengths are looked up
+    const uint32_t front = free_mask<kForkFirst>(P.counts, threadIdx.x * kForkFirst, 0, P.num_blocks, aligned);
     for (int64_t c0 = 0; c0 < P.n; c0 += kForkThreads) {
         const int64_t i = c0 + threadIdx.x;
         Child c = {-1, 0, 0, -1};
@@ -114,10 +117,13 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_take_kernel(const ForkPa
         const int rank = block_scan<kForkThreads>(need ? 1 : 0, part, wanted);
         int found = 0;
         if (threadIdx.x == 0) next_from = wanted ? P.num_blocks : from;
-        for (int64_t base = from & ~(int64_t)(kForkPages - 1); base < P.num_blocks && found < wanted;
-             base += (int64_t)kForkThreads * kForkPages) {
-            const int64_t mine = base + (int64_t)threadIdx.x * kForkPages;
-            uint32_t m = free_mask<kForkPages>(P.counts, mine, from, P.num_blocks, aligned);
+        int per = kForkFirst;
+        for (int64_t base = from & ~(int64_t)(kForkPages - 1); base < P.num_blocks && found < wanted; base += (int64_t)kForkThreads * per) {
+            if (base != (from & ~(int64_t)(kForkPages - 1))) per = kForkPages;
+            const int64_t mine = base + (int64_t)threadIdx.x * per;
+            uint32_t m = per == kForkPages ? free_mask<kForkPages>(P.counts, mine, from, P.num_blocks, aligned)
+                         : base == 0 && from == 0 ? front
+                                                  : free_mask<kForkFirst>(P.counts, mine, from, P.num_blocks, aligned);
             int total;
             int at = found + block_scan<kForkThreads>(__popc(m), part, total);
             while (m && at < wanted) {
@@ -141,25 +147,60 @@ __global__ void __launch_bounds__(kForkThreads) kv_fork_take_kernel(const ForkPa
     }
 }
 
+constexpr int kForkEntries = 8;
+// Entries j0, j0 + step, ... (kForkEntries of them) of child i: the loads first, so that they are under way together.
+__device__ __forceinline__ void fork_entries(const ForkParams& P, const Child& c, int64_t own, int64_t i, int64_t j0, int step) {
+    const bool dropped = c.parent < 0 || (c.page >= 0 && own < 0);  // no parent, or no page was left
+    const int64_t* row = P.table + (c.parent < 0 ? 0 : c.parent) * P.bt_s;
+    const int64_t shared = dropped ? 0 : c.full, last = dropped || !c.rest ? -1 : c.full;
+    int64_t e[kForkEntries];
+#pragma unroll
+    for (int x = 0; x < kForkEntries; ++x) {
+        const int64_t j = j0 + x * step;
+        e[x] = -1;
+        if (j < shared || (j == last && c.page < 0)) e[x] = row[j];
+        else if (j == last) e[x] = own;
+    }
+#pragma unroll
+    for (int x = 0; x < kForkEntries; ++x) {
+        const int64_t j = j0 + x * step;
+        if (j >= P.max_blocks) break;
+        if (j < shared && e[x] >= 0 && e[x] < P.num_blocks) atomicAdd(P.counts + e[x], 1);
+        P.child[i * P.max_blocks + j] = e[x];
+    }
+}
+
+// Small forks in one launch: a cluster whose first CTA hands out the pages and whose warps then take the children in turn.
+// (Two launches cost the host 4 us more, which is what a small fork takes.)
+constexpr int kForkCluster = 8;
+__global__ void __cluster_dims__(kForkCluster, 1, 1) __launch_bounds__(kForkThreads) kv_fork_small_kernel(const ForkParams P) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31, warps = kForkCluster * kForkThreads / 32;
+    const int64_t first = blockIdx.x * (kForkThreads / 32) + (threadIdx.x >> 5);
+    Child c = {-1, 0, 0, -1};
+    if (first < P.n) c = child_of(P, first);
+    if (blockIdx.x == 0) fork_take(P);
+    cooperative_groups::this_cluster().sync();  // also makes the pages visible to the other CTAs
+    for (int64_t i = first; i < P.n; i += warps) {
+        if (i != first) c = child_of(P, i);
+        const int64_t own = *(volatile int64_t*)(P.dst + i);
+        for (int64_t j = lane; j < P.max_blocks; j += 32 * kForkEntries) fork_entries(P, c, own, i, j, 32);
+    }
+}
+// Large ones in two.
+__global__ void __launch_bounds__(kForkThreads) kv_fork_take_kernel(const ForkParams P) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    fork_take(P);
+}
 __global__ void __launch_bounds__(256) kv_fork_table_kernel(const ForkParams P) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int64_t i = blockIdx.x;
     const Child c = child_of(P, i);
-    const int64_t own = P.dst[i];
-    const bool dropped = c.parent < 0 || (c.page >= 0 && own < 0);  // no parent, or no page was left
-    for (int64_t j = blockIdx.y * 256 + threadIdx.x; j < P.max_blocks; j += (int64_t)gridDim.y * 256) {
-        int64_t e = -1;
-        if (!dropped) {
-            if (j < c.full) {
-                e = P.table[c.parent * P.bt_s + j];
-                if (e >= 0 && e < P.num_blocks) atomicAdd(P.counts + e, 1);
-            } else if (j == c.full && c.rest) {
-                e = c.page >= 0 ? own : P.table[c.parent * P.bt_s + j];
-            }
-        }
-        P.child[i * P.max_blocks + j] = e;
-    }
+    constexpr int kStep = 256 * kForkEntries;
+    for (int64_t j = blockIdx.y * kStep + threadIdx.x; j < P.max_blocks; j += (int64_t)gridDim.y * kStep) fork_entries(P, c, P.dst[i], i, j, 256);
 }
 
 // ---- free -------------------------------------------------------------------------------------------
@@ -186,32 +227,37 @@ __global__ void __launch_bounds__(256) kv_free_kernel(int64_t* table, int64_t bt
 // one as of the other, and the last live page goes to the first hole.
 constexpr int kCompactThreads = 256, kCompactPages = 16, kCompactChunk = kCompactThreads * kCompactPages;
 
-__global__ void __launch_bounds__(kCompactThreads) kv_compact_count_kernel(const int32_t* counts, int64_t num, int32_t* chunk) {
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
+struct CompactParams {
+    int32_t* counts;
+    int64_t num;
+    int32_t* chunk;   // live pages of every kCompactChunk pages
+    int64_t *map, *src, *dst;
+    int32_t* n_moves;
+    int64_t* table;
+    int64_t bt_s, batch, max_blocks;
+    int chunks;
+};
+
+__device__ __forceinline__ void compact_count(const CompactParams& P, int g) {
     __shared__ int part[32];
-    const int64_t base = blockIdx.x * (int64_t)kCompactChunk + threadIdx.x * kCompactPages;
-    const int in = (int)(base >= num ? 0 : (num - base < kCompactPages ? num - base : kCompactPages));
-    const uint32_t m = free_mask<kCompactPages>(counts, base, 0, num, ((uintptr_t)counts & 15) == 0);
+    const int64_t base = g * (int64_t)kCompactChunk + threadIdx.x * kCompactPages;
+    const int in = (int)(base >= P.num ? 0 : (P.num - base < kCompactPages ? P.num - base : kCompactPages));
+    const uint32_t m = free_mask<kCompactPages>(P.counts, base, 0, P.num, ((uintptr_t)P.counts & 15) == 0);
     int total;
     block_scan<kCompactThreads>(in - __popc(m), part, total);
-    if (threadIdx.x == 0) chunk[blockIdx.x] = total;
+    if (threadIdx.x == 0) P.chunk[g] = total;
 }
 
-__global__ void __launch_bounds__(kCompactThreads) kv_compact_place_kernel(const int32_t* counts, int64_t num,
-                                                                           const int32_t* chunk, int64_t* map, int64_t* src,
-                                                                           int64_t* dst, int32_t* n_moves) {
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
+__device__ __forceinline__ void compact_place(const CompactParams& P, int g) {
     __shared__ int part[32];
-    const int64_t base = blockIdx.x * (int64_t)kCompactChunk + threadIdx.x * kCompactPages;
-    const int in = (int)(base >= num ? 0 : (num - base < kCompactPages ? num - base : kCompactPages));
-    const uint32_t m = free_mask<kCompactPages>(counts, base, 0, num, ((uintptr_t)counts & 15) == 0);
+    const int64_t base = g * (int64_t)kCompactChunk + threadIdx.x * kCompactPages;
+    const int in = (int)(base >= P.num ? 0 : (P.num - base < kCompactPages ? P.num - base : kCompactPages));
+    const uint32_t m = free_mask<kCompactPages>(P.counts, base, 0, P.num, ((uintptr_t)P.counts & 15) == 0);
     int all = 0, below = 0, unused;
-    for (int g = threadIdx.x; g < (int)gridDim.x; g += kCompactThreads) {
-        const int c = chunk[g];
+    for (int x = threadIdx.x; x < P.chunks; x += kCompactThreads) {
+        const int c = *(volatile int32_t*)(P.chunk + x);
         all += c;
-        if (g < (int)blockIdx.x) below += c;
+        if (x < g) below += c;
     }
     int live, before;
     block_scan<kCompactThreads>(all, part, live);
@@ -219,61 +265,85 @@ __global__ void __launch_bounds__(kCompactThreads) kv_compact_place_kernel(const
     int64_t L = before + block_scan<kCompactThreads>(in - __popc(m), part, unused);
     for (int j = 0; j < in; ++j) {
         const int64_t i = base + j;
-        if (i == live) *n_moves = (int)(live - L);
+        if (i == live) *P.n_moves = (int)(live - L);
         if (m >> j & 1) {
-            map[i] = -1;
-            if (i < live) dst[i - L] = i;
+            P.map[i] = -1;
+            if (i < live) P.dst[i - L] = i;
         } else {
             const int64_t rank = live - 1 - L;
-            map[i] = i < live ? i : -2 - rank;  // the hole's number, until the next kernel puts its page there
-            if (i >= live) src[rank] = i;
+            P.map[i] = i < live ? i : -2 - rank;  // the hole's number, until its page is put there
+            if (i >= live) P.src[rank] = i;
             ++L;
         }
     }
-    if (live == num && blockIdx.x == 0 && threadIdx.x == 0) *n_moves = 0;
+    if (live == P.num && g == 0 && threadIdx.x == 0) *P.n_moves = 0;
 }
 
-__global__ void __launch_bounds__(256) kv_compact_apply_kernel(int32_t* counts, int64_t* map, const int64_t* src,
-                                                               const int64_t* dst, const int32_t* n_moves, int64_t* table,
-                                                               int64_t bt_s, int64_t batch, int64_t max_blocks, int64_t num) {
+__device__ __forceinline__ void compact_apply(const CompactParams& P, int64_t first, int64_t step) {
+    const int64_t moves = *(volatile int32_t*)P.n_moves;
+    for (int64_t r = first; r < moves; r += step) {
+        const int64_t s = *(volatile int64_t*)(P.src + r), d = *(volatile int64_t*)(P.dst + r);
+        P.counts[d] = P.counts[s];
+        P.counts[s] = 0;
+        *(volatile int64_t*)(P.map + s) = d;
+    }
+    for (int64_t x = first; x < P.batch * P.max_blocks; x += step) {
+        const int64_t b = x / P.max_blocks;
+        int64_t* e = P.table + b * P.bt_s + (x - b * P.max_blocks);
+        const int64_t page = *e;
+        if (page < 0 || page >= P.num) continue;
+        const int64_t to = *(volatile int64_t*)(P.map + page);  // either form of a moved page's entry will do
+        *e = to < -1 ? *(volatile int64_t*)(P.dst - 2 - to) : to;
+    }
+}
+
+// Small pools in one launch of one cluster; large ones in three.
+constexpr int kCompactCluster = 8;
+constexpr int64_t kSmallCompact = 1 << 15;  // pages, and table entries
+__global__ void __cluster_dims__(kCompactCluster, 1, 1) __launch_bounds__(kCompactThreads) kv_compact_small_kernel(const CompactParams P) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
-    const int64_t step = (int64_t)gridDim.x * 256, first = blockIdx.x * (int64_t)256 + threadIdx.x;
-    const int64_t moves = *n_moves;
-    for (int64_t r = first; r < moves; r += step) {
-        const int64_t s = src[r], d = dst[r];
-        counts[d] = counts[s];
-        counts[s] = 0;
-        *(volatile int64_t*)(map + s) = d;
-    }
-    for (int64_t x = first; x < batch * max_blocks; x += step) {
-        const int64_t b = x / max_blocks;
-        int64_t* e = table + b * bt_s + (x - b * max_blocks);
-        const int64_t page = *e;
-        if (page < 0 || page >= num) continue;
-        const int64_t to = *(volatile int64_t*)(map + page);  // either form of a moved page's entry will do
-        *e = to < -1 ? dst[-2 - to] : to;
-    }
+    for (int g = blockIdx.x; g < P.chunks; g += kCompactCluster) compact_count(P, g);
+    cooperative_groups::this_cluster().sync();
+    for (int g = blockIdx.x; g < P.chunks; g += kCompactCluster) compact_place(P, g);
+    cooperative_groups::this_cluster().sync();
+    compact_apply(P, blockIdx.x * (int64_t)kCompactThreads + threadIdx.x, kCompactCluster * kCompactThreads);
+}
+__global__ void __launch_bounds__(kCompactThreads) kv_compact_count_kernel(const CompactParams P) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    compact_count(P, blockIdx.x);
+}
+__global__ void __launch_bounds__(kCompactThreads) kv_compact_place_kernel(const CompactParams P) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    compact_place(P, blockIdx.x);
+}
+__global__ void __launch_bounds__(kCompactThreads) kv_compact_apply_kernel(const CompactParams P) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    compact_apply(P, blockIdx.x * (int64_t)kCompactThreads + threadIdx.x, (int64_t)gridDim.x * kCompactThreads);
 }
 
 // ---- copies -----------------------------------------------------------------------------------------
 constexpr int kCopyLayers = 64;  // cache pairs of one launch: their addresses travel as kernel arguments
-struct CopyParams {
+struct Scales { float* of[2 * kCopyLayers]; };
+struct NoScales {};
+template <typename S> struct CopyParams {
     void* cache[2 * kCopyLayers];
-    float* scales[2 * kCopyLayers];
+    S scales;
     const int64_t *src, *dst;
     const int32_t *rows, *n_moves;
     int64_t n_pairs, num_blocks;
     int64_t sblk, sh, spos;  // in vectors
     int tensors, heads, vpr, block_size, strips;
     bool linear;             // a head's positions follow one another without a gap
-    bool has_scales;
 };
 
 // A warp copies a strip of 32*PER vectors of one head's positions of one page: every lane has all its loads
 // under way before the first store.
-template <typename VEC, int PER>
-__global__ void __launch_bounds__(256) kv_copy_pages_kernel(const CopyParams P) {
+template <typename VEC, int PER, typename S>
+__global__ void __launch_bounds__(256) kv_copy_pages_kernel(const CopyParams<S> P) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -327,16 +397,59 @@ __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const CopyParams P) 
                 if (v < end) { const int64_t at = v / P.vpr; to[at * P.spos + (v - at * P.vpr)] = x[k]; }
             }
         }
-        if (P.has_scales && strip == 0) {
-            float* sc = P.scales[t];
-            for (int r = lane; r < rows; r += 32)
-                sc[(dst * P.heads + h) * P.block_size + r] = sc[(src * P.heads + h) * P.block_size + r];
+        if constexpr (sizeof(S) == sizeof(Scales)) {
+            float* sc = P.scales.of[t];
+            if (strip == 0)
+                for (int r = lane; r < rows; r += 32)
+                    sc[(dst * P.heads + h) * P.block_size + r] = sc[(src * P.heads + h) * P.block_size + r];
         }
     }
 }
 
 int done(cudaError_t e, const char* name) {
     if (e != cudaSuccess) { cudaGetLastError(); return fail(RFX_CUDA_ERROR, "%s: %s", name, cudaGetErrorString(e)); }
+    return check_launch(name);
+}
+
+
+template <typename S> int copy_impl(const RfxKvCopyArgs* a, size_t vec, size_t e, const char* name) {
+    const int64_t per = (int64_t)(vec / e);
+    CopyParams<S> P;
+    P.src = a->src_pages; P.dst = a->dst_pages; P.rows = a->copy_rows; P.n_moves = a->n_moves;
+    P.n_pairs = a->n_pairs; P.num_blocks = a->num_blocks;
+    P.sblk = a->cache_stride_blk / per; P.sh = a->cache_stride_h / per; P.spos = a->cache_stride_pos / per;
+    P.heads = (int)a->num_kv_heads; P.vpr = (int)((size_t)a->head_dim * e / vec); P.block_size = (int)a->block_size;
+    P.linear = P.spos == P.vpr;
+    constexpr int PER = 8;
+    const int64_t strips = ceil_div<int64_t>((int64_t)P.vpr * P.block_size, 32 * PER);
+    RFX_REQUIRE(strips < (1ll << 31), "%s: a page of %lld positions x %lld elements is too large", name,
+                (long long)a->block_size, (long long)a->head_dim);
+    P.strips = (int)strips;
+    cudaStream_t s = as_stream(a->stream);
+    for (int64_t l0 = 0; l0 < a->n_layers; l0 += kCopyLayers) {
+        const int m = (int)(a->n_layers - l0 < kCopyLayers ? a->n_layers - l0 : kCopyLayers);
+        P.tensors = 2 * m;
+        for (int l = 0; l < m; ++l) {
+            P.cache[2 * l] = a->k_caches[l0 + l];
+            P.cache[2 * l + 1] = a->v_caches[l0 + l];
+            if constexpr (sizeof(S) == sizeof(Scales)) {
+                P.scales.of[2 * l] = a->k_scales[l0 + l];
+                P.scales.of[2 * l + 1] = a->v_scales[l0 + l];
+            }
+        }
+        const int64_t items = P.n_pairs * P.tensors * (int64_t)P.heads * P.strips;
+        int64_t blocks = ceil_div<int64_t>(items, 8);
+        if (blocks > (int64_t)sm_count() * 8) blocks = (int64_t)sm_count() * 8;
+        cudaError_t le;
+        switch (vec) {
+            case 16: le = launch_pdl(kv_copy_pages_kernel<uint4, PER, S>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
+            case 8: le = launch_pdl(kv_copy_pages_kernel<uint2, PER, S>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
+            case 4: le = launch_pdl(kv_copy_pages_kernel<uint32_t, PER, S>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
+            case 2: le = launch_pdl(kv_copy_pages_kernel<uint16_t, PER, S>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
+            default: le = launch_pdl(kv_copy_pages_kernel<uint8_t, PER, S>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
+        }
+        if (le != cudaSuccess) return done(le, name);
+    }
     return check_launch(name);
 }
 
@@ -361,10 +474,14 @@ extern "C" int rfx_kv_fork(const RfxKvForkArgs* a) {
     ForkParams P = {a->block_table, a->context_lens, a->parents, a->ref_counts, a->child_table, a->src_pages, a->dst_pages,
                     a->copy_rows, a->n_children, a->batch, a->max_blocks, a->bt_stride_b, a->num_blocks, (int)a->block_size};
     cudaStream_t s = as_stream(a->stream);
+    // One launch up to 32 K table entries; behind that the eight SMs of a cluster are too few (131 K entries with 65 K pages shared:
+    // 21 us, two launches 12).
+    if (a->n_children * a->max_blocks <= (1ll << 15))
+        return done(launch_pdl(kv_fork_small_kernel, dim3(kForkCluster), dim3(kForkThreads), 0, s, P), name);
     cudaError_t e = launch_pdl(kv_fork_take_kernel, dim3(1), dim3(kForkThreads), 0, s, P);
     if (e != cudaSuccess) return done(e, name);
     if (a->max_blocks > 0) {
-        int64_t y = ceil_div<int64_t>(a->max_blocks, 256);
+        int64_t y = ceil_div<int64_t>(a->max_blocks, 256 * kForkEntries);
         if (y > 64) y = 64;
         e = launch_pdl(kv_fork_table_kernel, dim3((unsigned)a->n_children, (unsigned)y), dim3(256), 0, s, P);
     }
@@ -406,18 +523,19 @@ extern "C" int rfx_kv_compact(const RfxKvCompactArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
     cudaStream_t s = as_stream(a->stream);
-    int32_t* chunk = (int32_t*)a->workspace;
-    const unsigned g = (unsigned)ceil_div<int64_t>(a->num_blocks, kCompactChunk);
-    cudaError_t e = launch_pdl(kv_compact_count_kernel, dim3(g), dim3(kCompactThreads), 0, s, a->ref_counts, a->num_blocks, chunk);
+    const int64_t g = ceil_div<int64_t>(a->num_blocks, kCompactChunk), entries = a->batch * a->max_blocks;
+    const CompactParams P = {a->ref_counts, a->num_blocks, (int32_t*)a->workspace, a->page_map, a->src_pages, a->dst_pages, a->n_moves,
+                             a->block_table, a->bt_stride_b, a->batch, a->max_blocks, (int)g};
+    if (a->num_blocks <= kSmallCompact && entries <= kSmallCompact)
+        return done(launch_pdl(kv_compact_small_kernel, dim3(kCompactCluster), dim3(kCompactThreads), 0, s, P), name);
+    cudaError_t e = launch_pdl(kv_compact_count_kernel, dim3((unsigned)g), dim3(kCompactThreads), 0, s, P);
     if (e != cudaSuccess) return done(e, name);
-    e = launch_pdl(kv_compact_place_kernel, dim3(g), dim3(kCompactThreads), 0, s, a->ref_counts, a->num_blocks, chunk,
-                   a->page_map, a->src_pages, a->dst_pages, a->n_moves);
+    e = launch_pdl(kv_compact_place_kernel, dim3((unsigned)g), dim3(kCompactThreads), 0, s, P);
     if (e != cudaSuccess) return done(e, name);
-    const int64_t most = a->batch * a->max_blocks > a->num_blocks / 2 ? a->batch * a->max_blocks : a->num_blocks / 2;
-    int64_t blocks = ceil_div<int64_t>(most < 1 ? 1 : most, 256);
+    const int64_t most = entries > a->num_blocks / 2 ? entries : a->num_blocks / 2;
+    int64_t blocks = ceil_div<int64_t>(most < 1 ? 1 : most, kCompactThreads);
     if (blocks > (int64_t)sm_count() * 8) blocks = (int64_t)sm_count() * 8;
-    e = launch_pdl(kv_compact_apply_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a->ref_counts, a->page_map, a->src_pages,
-                   a->dst_pages, a->n_moves, a->block_table, a->bt_stride_b, a->batch, a->max_blocks, a->num_blocks);
+    e = launch_pdl(kv_compact_apply_kernel, dim3((unsigned)blocks), dim3(kCompactThreads), 0, s, P);
     return done(e, name);
 }
 
@@ -452,40 +570,6 @@ extern "C" int rfx_kv_copy_pages(const RfxKvCopyArgs* a) {
         return true;
     };
     while (vec > e && !fits(vec)) vec /= 2;
-    const int64_t per = (int64_t)(vec / e);
-    CopyParams P = {};
-    P.src = a->src_pages; P.dst = a->dst_pages; P.rows = a->copy_rows; P.n_moves = a->n_moves;
-    P.n_pairs = a->n_pairs; P.num_blocks = a->num_blocks;
-    P.sblk = a->cache_stride_blk / per; P.sh = a->cache_stride_h / per; P.spos = a->cache_stride_pos / per;
-    P.heads = (int)a->num_kv_heads; P.vpr = (int)(row / vec); P.block_size = (int)a->block_size;
-    P.linear = P.spos == P.vpr;
-    P.has_scales = a->kv_int8 != 0;
-    constexpr int PER = 8;
-    const int64_t strips = ceil_div<int64_t>((int64_t)P.vpr * P.block_size, 32 * PER);
-    RFX_REQUIRE(strips < (1ll << 31), "%s: a page of %lld positions x %lld elements is too large", name,
-                (long long)a->block_size, (long long)a->head_dim);
-    P.strips = (int)strips;
-    cudaStream_t s = as_stream(a->stream);
-    for (int64_t l0 = 0; l0 < a->n_layers; l0 += kCopyLayers) {
-        const int m = (int)(a->n_layers - l0 < kCopyLayers ? a->n_layers - l0 : kCopyLayers);
-        P.tensors = 2 * m;
-        for (int l = 0; l < m; ++l) {
-            P.cache[2 * l] = a->k_caches[l0 + l];
-            P.cache[2 * l + 1] = a->v_caches[l0 + l];
-            if (P.has_scales) { P.scales[2 * l] = a->k_scales[l0 + l]; P.scales[2 * l + 1] = a->v_scales[l0 + l]; }
-        }
-        const int64_t items = P.n_pairs * P.tensors * (int64_t)P.heads * P.strips;
-        int64_t blocks = ceil_div<int64_t>(items, 8);
-        if (blocks > (int64_t)sm_count() * 8) blocks = (int64_t)sm_count() * 8;
-        cudaError_t le;
-        switch (vec) {
-            case 16: le = launch_pdl(kv_copy_pages_kernel<uint4, PER>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
-            case 8: le = launch_pdl(kv_copy_pages_kernel<uint2, PER>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
-            case 4: le = launch_pdl(kv_copy_pages_kernel<uint32_t, PER>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
-            case 2: le = launch_pdl(kv_copy_pages_kernel<uint16_t, PER>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
-            default: le = launch_pdl(kv_copy_pages_kernel<uint8_t, PER>, dim3((unsigned)blocks), dim3(256), 0, s, P); break;
-        }
-        if (le != cudaSuccess) return done(le, name);
-    }
-    return check_launch(name);
+    if (a->kv_int8) return copy_impl<Scales>(a, vec, e, name);
+    return copy_impl<NoScales>(a, vec, e, name);
 }

@@ -197,12 +197,12 @@ template <typename F> __device__ __forceinline__ void sort_by_bins(Shared& s, in
     __syncthreads();
 }
 
-// A key that at least `count` <= kGroups of the CTA's group maxima reach (a key of -inf or below, if fewer groups hold
-// logits): the count-th largest with its last bits cleared, ten bits below the highest in which two maxima differ.
-// Leaves it, the largest key and s.n in s.picked. One histogram over those ten bits and a scan: four barriers.
-// (One warp that searched bit by bit took 2 us.)
-__device__ __forceinline__ void select(Shared& s, float most0, float most1, int count) {
-    static_assert(kGroups == 1024 && kThreads == 512, "ten bits, two bins a thread");
+// A key that at least `count` <= kGroups of the CTA's group maxima reach, or below which no logit weighs anything, whichever is
+// larger; a little below the count-th largest. Leaves it, the largest key and s.n in s.picked. One histogram of 1024 bins
+// over the maxima between the largest and `range` below it (where weights end: a bin over the bits of their keys is
+// coarse when some are negative or masked) and a scan: four barriers. (One warp that searched bit by bit took 2 us.)
+__device__ __forceinline__ void select(Shared& s, float most0, float most1, int count, float range) {
+    static_assert(kGroups == 1024 && kThreads == 512, "two bins a thread");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t k0 = key_of(most0), k1 = key_of(most1);
     reinterpret_cast<uint2*>(s.group)[threadIdx.x] = make_uint2(0, 0);
@@ -210,13 +210,17 @@ __device__ __forceinline__ void select(Shared& s, float most0, float most1, int 
     if (lane == 0) s.part[warp] = (u64)h << 32 | l;
     __syncthreads();
     const u64 hl = s.part[lane & (kWarps - 1)];
-    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(hl >> 32));
-    const uint32_t low = __reduce_min_sync(0xffffffffu, (uint32_t)hl);
-    const int first = high == low ? 0 : 31 - __clz(high ^ low), shift = max(0, first - 9);
-    const uint32_t base = first == 31 ? 0 : high >> (first + 1) << (first + 1);
-    atomicAdd(&s.group[1023 - ((k0 - base) >> shift)], 1u);  // the largest in front
-    atomicAdd(&s.group[1023 - ((k1 - base) >> shift)], 1u);
-    if (threadIdx.x == 0) { s.picked[1] = high; s.picked[2] = (uint32_t)s.n; }
+    const uint32_t high_key = __reduce_max_sync(0xffffffffu, (uint32_t)(hl >> 32));
+    const float high = value_of(high_key), low = fmaxf(fmaxf(value_of(__reduce_min_sync(0xffffffffu, (uint32_t)hl)), high - range), kLowest);
+    const float width = fminf(high - low, -kLowest), scale = width > 0.f ? 1023.f / width : 0.f;
+    // (an infinite maximum: nothing else weighs; none at all: low is above it, and no bin is filled)
+    if (most0 >= low && high < INFINITY) atomicAdd(&s.group[min(1023, (int)(fminf(high - most0, -kLowest) * scale))], 1u);
+    if (most1 >= low && high < INFINITY) atomicAdd(&s.group[min(1023, (int)(fminf(high - most1, -kLowest) * scale))], 1u);
+    if (threadIdx.x == 0) {
+        s.picked[0] = high < INFINITY ? key_of(low) : high_key;
+        s.picked[1] = high_key;
+        s.picked[2] = (uint32_t)s.n;
+    }
     __syncthreads();
     const uint2 m = reinterpret_cast<const uint2*>(s.group)[threadIdx.x];
     const int own = (int)(m.x + m.y);
@@ -231,8 +235,10 @@ __device__ __forceinline__ void select(Shared& s, float most0, float most1, int 
     const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? (int)s.part[lane & (kWarps - 1)] : 0);
     const int before = ahead + x - own;
     if (before < count && before + own >= count) {
-        const uint32_t bin = 2 * threadIdx.x + (before + (int)m.x >= count ? 0 : 1);
-        s.picked[0] = base + ((1023 - bin) << shift);
+        const int bin = 2 * threadIdx.x + (before + (int)m.x >= count ? 0 : 1);
+        // the bin's lower end, further down than any rounding
+        const float end = high - (float)(bin + 1) / scale - 1e-6f * (fabsf(high) + width);
+        if (scale > 0.f && end > low) s.picked[0] = key_of(end);
     }
     __syncthreads();
 }
@@ -906,7 +912,7 @@ template <typename T> struct Row {
 
     // Streams the slice and leaves every logit that can be among the row's k largest in the CTAs' lists (or more than
     // kCap in one, which says that the list will not do). Sets `top`.
-    __device__ __forceinline__ void stream(int k) {
+    __device__ __forceinline__ void stream(int k, float range) {
         const int share = (k + ranks - 1) / ranks;  // so many of every CTA together are k
         float most[2] = {-INFINITY, -INFINITY};
         uint32_t own = 0;
@@ -927,6 +933,9 @@ template <typename T> struct Row {
         } else {
             float bound = kLowest;
             int j0 = threadIdx.x, seen = kStep, renew = kStep;  // renew: chunks seen when the bound is renewed next
+            // A renewal costs the CTA a microsecond without work. About 1.1 k logits come in between two of them at a
+            // doubling, three times as many at a fourfold count: small lists take that.
+            const int grow = k <= kCap / 9 ? 4 : 2;
             bool here = inside(0);
             if (here) fetch<true>(c, j0); else fetch<false>(c, j0);
             auto batch = [&](const Chunk<T> (&c)[kBatch], Chunk<T> (&next)[kBatch]) {
@@ -935,10 +944,10 @@ template <typename T> struct Row {
                 else if (seen < nvec) fetch<false>(next, j0 + kStep);
                 if (here) look(c, j0, whole_batch); else look(c, j0, ends);
                 if (seen >= renew || seen >= nvec) {
-                    select(s, most[0], most[1], k);
+                    select(s, most[0], most[1], k, range);
                     own = s.picked[0];
                     bound = bound_of(own);
-                    renew = 2 * seen;
+                    renew = grow * seen;
                     const int n = (int)s.picked[2];  // s.n itself is on the move again
                     if (n > kCap / 2 && n <= kCap) drop_below(own);
                 }
@@ -953,7 +962,7 @@ template <typename T> struct Row {
             while (batch(c, other) && batch(other, c)) {}
             __syncthreads();
         }
-        if (one || ranks > 1) select(s, most[0], most[1], share);
+        if (one || ranks > 1) select(s, most[0], most[1], share, range);
         uint32_t bound = s.picked[0];
         const u64 o = exchange((u64)s.picked[1] << 32 | bound);
         const bool lane_in = (threadIdx.x & 31) < ranks;
@@ -1029,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     cluster.barrier_wait(std::move(started));
 
     if (by_list) {
-        r.stream(k);
+        r.stream(k, (float)((P.shift + 2) * 0.6931471805599454 * t));  // weights end before that far below the largest
         const int n = r.top == -INFINITY ? 0 : r.collect();
         if (r.top > -INFINITY && n <= kCap) {
             // rank 0 has pulled the lists: the others may leave

@@ -19,7 +19,7 @@ Page bookkeeping (additive; the reference leaves it to its caller), all of it on
 """
 from __future__ import annotations
 
-import ctypes as C
+from array import array
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
@@ -216,7 +216,7 @@ def kv_fork(
     parents = _int32_vector(name, "parents", parents)
     n = parents.shape[0]
     child = block_table.new_empty((n, max_blocks))
-    src, dst = block_table.new_empty((2, n))
+    src, dst = block_table.new_empty(n), block_table.new_empty(n)
     rows = parents.new_empty(n)
     _fork(index, block_table.data_ptr(), context_lens.data_ptr(), parents.data_ptr(), ref_counts.data_ptr(),
           child.data_ptr(), src.data_ptr(), dst.data_ptr(), rows.data_ptr(),
@@ -263,7 +263,7 @@ def kv_compact(
     _check_table(name, block_table, ref_counts)
     num = ref_counts.shape[0]
     page_map = block_table.new_empty(num)
-    src, dst = block_table.new_empty((2, num // 2 + 1))
+    src, dst = block_table.new_empty(num // 2 + 1), block_table.new_empty(num // 2 + 1)
     need = int(N.lib().rfx_kv_compact_workspace_bytes(num))
     words = ref_counts.new_empty(64 + need // 4)  # the number of moves stands in front of the scratch
     count = words[:1]
@@ -275,6 +275,11 @@ def kv_compact(
 
 def _layers(t):
     return [t] if isinstance(t, torch.Tensor) else list(t)
+
+
+def _pointers(tensors):
+    """The tensors' addresses as a C array."""
+    return array("Q", [t.data_ptr() for t in tensors])
 
 
 def kv_copy_pages(
@@ -301,11 +306,13 @@ def kv_copy_pages(
     src, dst, rows, count = moves
     first = ks[0]
     index = N.same_device(name, first, src, dst, rows, count, *ks, *vs)
-    _check_pool(name, first, vs[0])
     shape, strides, dtype = first.shape, first.stride(), first.dtype
+    if len(shape) != 4 or strides[3] != 1:
+        raise ValueError(f"{name}: caches must be [num_blocks, num_heads, block_size, head_dim], the last axis contiguous; "
+                         f"got {tuple(shape)}, strides {strides}")
     for t in ks + vs:
         if t is not first and (t.shape != shape or t.stride() != strides or t.dtype != dtype):
-            raise ValueError(f"{name}: the caches of all layers must share one shape, stride pattern and dtype")
+            raise ValueError(f"{name}: all caches must share one shape, stride pattern and dtype")
     if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.dim() != 1 or dst.shape != src.shape:
         raise ValueError(f"{name}: moves.src and moves.dst must be int64 [n]")
     n = src.shape[0]
@@ -315,8 +322,7 @@ def kv_copy_pages(
     if count is not None and (count.dtype != torch.int32 or count.numel() != 1):
         raise ValueError(f"{name}: moves.count must be one int32")
     L = len(ks)
-    array = N.vp * L
-    k_ptrs, v_ptrs = array(*[t.data_ptr() for t in ks]), array(*[t.data_ptr() for t in vs])
+    k_ptrs, v_ptrs = _pointers(ks), _pointers(vs)
     int8, k_scale_ptrs, v_scale_ptrs = 0, None, None
     if dtype == torch.int8:
         int8 = 1
@@ -329,9 +335,9 @@ def kv_copy_pages(
         for t in sk + sv:
             if t.dtype != torch.float32 or t.shape != shape[:3] or not t.is_contiguous():
                 raise ValueError(f"{name}: scales must be contiguous float32 {list(shape[:3])}")
-        k_scale_ptrs, v_scale_ptrs = array(*[t.data_ptr() for t in sk]), array(*[t.data_ptr() for t in sv])
-    _copy(index, C.addressof(k_ptrs), C.addressof(v_ptrs), C.addressof(k_scale_ptrs) if int8 else 0,
-          C.addressof(v_scale_ptrs) if int8 else 0, src.data_ptr(), dst.data_ptr(),
+        k_scale_ptrs, v_scale_ptrs = _pointers(sk), _pointers(sv)
+    _copy(index, k_ptrs.buffer_info()[0], v_ptrs.buffer_info()[0], k_scale_ptrs.buffer_info()[0] if int8 else 0,
+          v_scale_ptrs.buffer_info()[0] if int8 else 0, src.data_ptr(), dst.data_ptr(),
           0 if rows is None else rows.data_ptr(), 0 if count is None else count.data_ptr(),
           L, n, shape[1], shape[3], shape[0], shape[2], strides[0], strides[1], strides[2],
           0 if int8 else N.dtype_code(first), int8, N.stream_of(index))
