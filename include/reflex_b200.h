@@ -340,8 +340,8 @@ int rfx_online_softmax(const RfxSoftmaxArgs* a);
  *   uniform * their sum (uniform >= 1: the last of weight, below 0 or NaN: the first).
  * temperature <= 0 or NaN: the lowest index of the largest logit (above 0 it counts as 1e-20 at least). A row with nothing but -inf (or NaN) gives
  * -1; with +inf among its logits those share the mass. Every setting is a device array [batch], or with a
- * NULL pointer one number for all rows. Weights are exp in 64 bits, summed as whole multiples of 2^-S of the
- * largest, S = min(50, 62 - log2 vocab): the result depends on nothing but the arguments. vocab <= 2^24. */
+ * NULL pointer one number for all rows. Weights are computed to 2^-39 of themselves and summed as whole multiples
+ * of 2^-S of the largest, S = min(50, 62 - log2 vocab): the result depends on nothing but the arguments. vocab <= 2^24. */
 typedef struct {
     const void* logits;          /* [batch, vocab], row stride below, last dim contiguous */
     const float* uniform;        /* [batch], in [0, 1) */

@@ -6,9 +6,9 @@
 //   the token is the lowest index whose running sum of kept weights, in index order, exceeds u * their sum.
 //
 // The answer hangs on which side of a border a sum lies, so sums must not depend on the order in which
-// threads or CTAs run: a weight is exp() in 64 bits, rounded to a whole multiple of 2^-S with
-// S = min(50, 62 - log2 V), and added up as a 64-bit integer. Such sums are exact in any order; what a weight
-// loses (2^-S-1 of the largest, 2^-46 at 131072 tokens) is far below the distance of two borders.
+// threads or CTAs run: a weight is computed in 64 bits to 2^-39 of itself, rounded to a whole multiple of 2^-S with
+// S = min(50, 62 - log2 V), and added up as a 64-bit integer. Such sums are exact in any order; what a weight loses is far
+// below the distance of two borders (131072 tokens: a border in 3e-7 rows is that near the number drawn).
 //
 // A cluster of up to 8 CTAs takes a row, each a slice of it (one CTA a row in large batches). Two ways to the
 // answer, by the row's settings:
@@ -81,7 +81,7 @@ struct __align__(16) Shared {
     u64 part[kWarps];
     u64 ends[2][kWarps];
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
-    u64 shares[kMaxCluster][kMaxCluster];  // [CTA][share of the bins]: masses of that CTA's logits
+    u64 shares[2][kMaxCluster][kMaxCluster];  // [top-k, top-p][CTA][share of the bins]: what that CTA's logits add to it
     u64 found[3];              // what one CTA tells all: a bin and the sum before it, a cut
     double power[32];          // as in SampleParams
     uint32_t picked[3];        // of select(): the bound, the largest key, n before it
@@ -212,7 +212,7 @@ __device__ __forceinline__ void select(Shared& s, float most0, float most1, int 
     const u64 hl = s.part[lane & (kWarps - 1)];
     const uint32_t high_key = __reduce_max_sync(0xffffffffu, (uint32_t)(hl >> 32));
     const float high = value_of(high_key), low = fmaxf(fmaxf(value_of(__reduce_min_sync(0xffffffffu, (uint32_t)hl)), high - range), kLowest);
-    const float width = fminf(high - low, -kLowest), scale = width > 0.f ? 1023.f / width : 0.f;
+    const float width = fminf(high - low, -kLowest), scale = width > 1e-30f ? 1023.f / width : 0.f;
     // (an infinite maximum: nothing else weighs; none at all: low is above it, and no bin is filled)
     if (most0 >= low && high < INFINITY) atomicAdd(&s.group[min(1023, (int)(fminf(high - most0, -kLowest) * scale))], 1u);
     if (most1 >= low && high < INFINITY) atomicAdd(&s.group[min(1023, (int)(fminf(high - most1, -kLowest) * scale))], 1u);
@@ -485,13 +485,13 @@ template <typename T> struct Row {
                 const int per = kWarps / ranks;
                 m = 0;
                 for (int w = 0; w < per; ++w) m += s.part[threadIdx.x * per + w];
-                for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s.shares[rank][threadIdx.x], r) = m;
+                for (int r = 0; r < ranks; ++r) *cg::this_cluster().map_shared_rank(&s.shares[MASS][rank][threadIdx.x], r) = m;
             }
         }
         cg::this_cluster().sync();
         u64 in_share = 0;
         if (lane < ranks)
-            for (int r = 0; r < ranks; ++r) in_share += s.shares[r][lane];
+            for (int r = 0; r < ranks; ++r) in_share += s.shares[MASS][r][lane];
         u64 total = warp_total(in_share);
         if (!MASS && total <= (u64)k) return;  // the border lies behind the last logit that weighs anything
         const u64 target = MASS ? target_of(p, total) : (u64)k;
@@ -773,7 +773,7 @@ template <typename T> struct Row {
             return draw_pairs(n, u, token);
         }
         // falling from the largest to the smallest listed
-        const float low = value_of(__reduce_min_sync(0xffffffffu, lowest_key(n)));
+        const float low = value_of(lowest_key(n));
         const float per_unit = top - low > 0.f ? (float)(kBins - 1) / fminf(top - low, 3.4e38f) : 0.f;
         sort_by_bins(s, n, [&](u64 e) {
             const float d = top - value_of((uint32_t)(e >> 32));
@@ -790,7 +790,7 @@ template <typename T> struct Row {
         __syncthreads();
         if ((threadIdx.x & 31) == 0) s.part[threadIdx.x >> 5] = low;
         __syncthreads();
-        return (uint32_t)s.part[threadIdx.x & (kWarps - 1)];
+        return __reduce_min_sync(0xffffffffu, (uint32_t)s.part[threadIdx.x & (kWarps - 1)]);
     }
     // The rest over a sorted list of at most PER * kThreads entries, PER neighbours a thread.
     template <int PER> __device__ __forceinline__ void finish_sorted(int n, float p, u64 least, float u, int64_t* token) {
