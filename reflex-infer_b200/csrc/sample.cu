@@ -315,17 +315,27 @@ template <typename T> struct Row {
         c.raw = reinterpret_cast<const uint4*>(stage)[j];
         return c;
     }
-    // f(chunk, index of its first logit) for the slice; what lies outside it reads as -inf
-    template <typename F> __device__ __forceinline__ void each_chunk(F f) const {
-        for (int j = threadIdx.x; j < nvec; j += kThreads) f(load(j), base + j * N);
-    }
-    // f(value, index) for the slice; what lies outside it reads as -inf
-    template <typename F> __device__ __forceinline__ void each(F f) const {
-        for (int j = threadIdx.x; j < nvec; j += kThreads) {
-            const Chunk<T> c = load(j);
-#pragma unroll
-            for (int e = 0; e < N; ++e) f(c.at(e), base + j * N + e);
+    // f(chunk, its number) for chunks from, from + step, ... below `to`; what lies outside the slice reads as -inf. The next
+    // chunk is on its way while one is worked on: where the slice is not staged it comes from L2.
+    template <typename F> __device__ __forceinline__ void chunks(int from, int to, int step, F f) const {
+        if (from >= to) return;
+        Chunk<T> c = load(from);
+        for (int j = from; j < to; j += step) {
+            Chunk<T> next;
+            if (j + step < to) next = load(j + step);
+            f(c, j);
+            c.raw = next.raw;
         }
+    }
+    template <typename F> __device__ __forceinline__ void each_chunk(F f) const {
+        chunks(threadIdx.x, nvec, kThreads, [&](const Chunk<T>& c, int j) { f(c, base + j * N); });
+    }
+    // f(value, index) for the slice
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        each_chunk([&](const Chunk<T>& c, int i0) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(c.at(e), i0 + e);
+        });
     }
     // The weight exp((v - top) / T) as a multiple of 2^-S, rounded to a whole number, for zero_below <= v <= top; and its
     // bin, the weight's distance from 1 in steps of 1/32 of a power of two. With 32 log2 of the weight = n + f, n whole and
@@ -612,8 +622,7 @@ template <typename T> struct Row {
         const int per = (nvec + kWarps - 1) / kWarps, from = warp * per, to = min(nvec, from + per);
         const u64 least = least_of(min_p);
         // the masses of a chunk's logits that stay; their sum
-        auto masses = [&](int j, u64 (&m)[N]) {
-            const Chunk<T> c = load(j);
+        auto masses = [&](const Chunk<T>& c, int j, u64 (&m)[N]) {
             u64 sum = 0;
             if (!(c.most() >= cut_value)) {
 #pragma unroll
@@ -630,10 +639,10 @@ template <typename T> struct Row {
             return sum;
         };
         u64 sum = 0;
-        for (int j = from + lane; j < to; j += 32) {
+        chunks(from + lane, to, 32, [&](const Chunk<T>& c, int j) {
             u64 m[N];
-            sum += masses(j, m);
-        }
+            sum += masses(c, j, m);
+        });
         const u64 all = warp_total(sum);
         __syncthreads();
         if (lane == 0) s.part[warp] = all;
@@ -653,7 +662,7 @@ template <typename T> struct Row {
             const int j = j0 + lane;
 #pragma unroll
             for (int e = 0; e < N; ++e) m[e] = 0;
-            if (j < to) own = masses(j, m);
+            if (j < to) own = masses(load(j), j, m);
             u64 x = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -1079,12 +1088,13 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
 
-    // CTAs of a row: one where the rows alone give every SM one (256 x 131072 fp32: 41.7 us, with two a row 57.6), else as many as
-    // give every SM two while a CTA keeps 8 logits or more a thread (64 x 131072 bf16: eight 46.9 us, four 52.2: rows
-    // differ in work by their settings, and finer pieces even that out).
+    // CTAs of a row: as many as give every SM one while a CTA keeps 8 logits or more a thread (256 x 131072 fp32, top-k: one a
+    // row 41.7 us, two 57.6). Settings given row by row give rows of unequal work; then twice as many, if one is not
+    // enough anyway (64 x 131072 bf16: mixed rows 40.2 us with eight a row, 48.1 with four; rows with top-k alone 21.0 and 14.8).
+    const bool unequal = a->temperature || a->top_k || a->top_p || a->min_p;
     int C = 1;
     auto slice_of = [&](int c) { return round_up<int64_t>(ceil_div<int64_t>(a->vocab, c), 8); };
-    while (C < kMaxCluster && a->batch < sm_count() && a->batch * C < 2 * sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
+    while (C < kMaxCluster && a->batch < sm_count() && a->batch * C < (unequal ? 2 : 1) * sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
     const int64_t slice = slice_of(C);
     const size_t bytes = round_up<size_t>((size_t)(slice + 8) * e, 16);
     const bool staged = bytes <= (a->batch * C > sm_count() ? kStageTwo : kStageMax);
