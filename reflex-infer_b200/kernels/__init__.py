@@ -8,7 +8,10 @@ Import names follow the reference's package (``README.md:117-125``):
     from kernels.attention import fused_attention
 
 plus the fused paged entry points in ``kernels.attention`` (``paged_decode``,
-``paged_attention``, ``rope_append``, ``paged_decode_step``, ``PagedWorkspace``).
+``paged_attention``, ``rope_append``, ``paged_decode_step``, ``PagedWorkspace``) and the operators of a
+serving step around them: ``kernels.rope.qk_norm_rope``, ``kernels.attention.qk_norm_rope_append``,
+``kernels.kv_cache.kv_fork`` / ``kv_free`` / ``kv_compact`` / ``kv_copy_pages`` and
+``kernels.softmax.sample_tokens``.
 Every function calls ``libreflex_b200.so`` through ``kernels._native``; there is no
 Triton, no backend dispatch and no CPU path.
 """
