@@ -106,12 +106,21 @@ __device__ __forceinline__ void fork_take(const ForkParams& P) {
     __shared__ int64_t next_from;
     const bool aligned = ((uintptr_t)P.counts & 15) == 0;
     int64_t from = 0;
-    // the first pages' counts are on their way while the children's lengths are looked up
-    const uint32_t front = free_mask<kForkFirst>(P.counts, threadIdx.x * kForkFirst, 0, P.num_blocks, aligned);
+    // No page that a child copies from is handed out, even if its count says that it is free.
+    Child mine_first = {-1, 0, 0, -1};
+    for (int64_t i = threadIdx.x; i < P.n; i += kForkThreads) {
+        const Child c = child_of(P, i);
+        if (c.page >= 0 && P.counts[c.page] <= 0) P.counts[c.page] = 1;
+        if (i < kForkThreads) mine_first = c;
+    }
+    __syncthreads();
     for (int64_t c0 = 0; c0 < P.n; c0 += kForkThreads) {
         const int64_t i = c0 + threadIdx.x;
-        Child c = {-1, 0, 0, -1};
-        if (i < P.n) c = child_of(P, i);
+        Child c = mine_first;
+        if (c0 > 0) {
+            c = {-1, 0, 0, -1};
+            if (i < P.n) c = child_of(P, i);
+        }
         const bool need = c.page >= 0;
         int wanted;
         const int rank = block_scan<kForkThreads>(need ? 1 : 0, part, wanted);
@@ -122,8 +131,7 @@ __device__ __forceinline__ void fork_take(const ForkParams& P) {
             if (base != (from & ~(int64_t)(kForkPages - 1))) per = kForkPages;
             const int64_t mine = base + (int64_t)threadIdx.x * per;
             uint32_t m = per == kForkPages ? free_mask<kForkPages>(P.counts, mine, from, P.num_blocks, aligned)
-                         : base == 0 && from == 0 ? front
-                                                  : free_mask<kForkFirst>(P.counts, mine, from, P.num_blocks, aligned);
+                                           : free_mask<kForkFirst>(P.counts, mine, from, P.num_blocks, aligned);
             int total;
             int at = found + block_scan<kForkThreads>(__popc(m), part, total);
             while (m && at < wanted) {

@@ -203,7 +203,8 @@ def kv_fork(
     appended. ``child_table`` is ``[n, max_blocks]`` int64, -1 behind the child's pages. Children take free
     pages in order; one for which none is left has ``moves.src >= 0`` and ``moves.dst < 0``, and it (and one
     whose parent is no row) gets a row of -1 and holds nothing. A parent may have any number of children;
-    it keeps its own pages until ``kv_free``.
+    it keeps its own pages until ``kv_free``. A page that a child copies from is never handed out (a count of
+    0 there, which says that nobody holds it, becomes 1).
     """
     N.check_backend(backend)
     name = "kv_fork"

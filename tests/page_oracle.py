@@ -9,8 +9,13 @@ def fork(table, lens, parents, counts, bs):
     table, lens, parents, rc = table.tolist(), lens.tolist(), parents.tolist(), counts.tolist()
     width = len(table[0]) if table else 0
     nb = len(rc)
+    for p in parents:  # what is copied from counts as held
+        if 0 <= p < len(table):
+            full, rest = divmod(min(max(lens[p], 0), width * bs), bs)
+            if rest and 0 <= table[p][full] < nb:
+                rc[table[p][full]] = max(rc[table[p][full]], 1)
     free = iter([p for p in range(nb) if rc[p] == 0])
-    child, src, dst, rows = [], [], [], []
+    child, src, dst, rows, shared = [], [], [], [], []
     for p in parents:
         row, s, d, r = [-1] * width, -1, -1, 0
         if 0 <= p < len(table):
@@ -30,12 +35,12 @@ def fork(table, lens, parents, counts, bs):
             if ok:
                 if d >= 0:
                     rc[d] = 1
-                for page in table[p][:full]:
-                    if 0 <= page < nb:
-                        rc[page] += 1
+                shared += [page for page in table[p][:full] if 0 <= page < nb]
             else:
                 row = [-1] * width
         child.append(row); src.append(s); dst.append(d); rows.append(r)
+    for page in shared:  # on top of what was handed out
+        rc[page] += 1
     return (torch.tensor(child, dtype=torch.int64).reshape(len(parents), width), torch.tensor(src, dtype=torch.int64),
             torch.tensor(dst, dtype=torch.int64), torch.tensor(rows, dtype=torch.int32), torch.tensor(rc, dtype=torch.int32))
 
