@@ -30,7 +30,7 @@ from typing import Optional
 import torch
 
 from .. import _native as N
-from ..rope import _norm_inputs
+from ..rope import _norm_inputs, _rows
 
 
 def _resolve_head_repeat(num_heads_q: int, num_heads_kv: int) -> int:
@@ -511,18 +511,12 @@ def qk_norm_rope_append(
         raise ValueError(f"{name}: positions are required")
     index = N.same_device(name, k_new, q, v_new, k_cache, v_cache, slot_mapping, positions, cos, sin, q_weight,
                           k_weight, q_out, k_scales, v_scales)
-    if k_new.stride(-1) != 1:
-        k_new = k_new.contiguous()
-    if v_new.stride(-1) != 1:
-        v_new = v_new.contiguous()
-    if q is not None and q.stride(-1) != 1:
-        q = q.contiguous()
-    cos, sin, positions, q_weight, k_weight = _norm_inputs(name, q, k_new, q_weight, k_weight, cos, sin, positions, eps)
+    n, hkv, D, hq, dtype, cos, sin, positions, q_weight, k_weight, f32 = _norm_inputs(
+        name, q, k_new, q_weight, k_weight, cos, sin, positions, eps)
     code = N.dtype_code(k_new)
-    shape, dtype, pool, strides = k_new.shape, k_new.dtype, k_cache.shape, k_cache.stride()
-    n, hkv, D = shape
-    if v_new.shape != shape or v_new.dtype != dtype:
-        raise ValueError(f"{name}: v_new must be like k_new, {tuple(shape)} in {dtype}")
+    pool, strides = k_cache.shape, k_cache.stride()
+    if v_new.shape != (n, hkv, D) or v_new.dtype != dtype:
+        raise ValueError(f"{name}: v_new must be like k_new, {(n, hkv, D)} in {dtype}")
     if len(pool) != 4 or v_cache.shape != pool or v_cache.stride() != strides:
         raise ValueError(f"{name}: caches must both be [num_blocks, H_kv, block_size, D] with one stride pattern")
     nb, ch, bs, cd = pool
@@ -530,8 +524,8 @@ def qk_norm_rope_append(
         raise ValueError(f"{name}: input heads/head_dim {(hkv, D)} do not match the cache {(ch, cd)}")
     if strides[3] != 1:
         raise ValueError(f"{name}: the head_dim axis of the caches must be contiguous")
-    kv_int8 = 0
-    if k_cache.dtype == torch.int8:
+    kv_int8, cache_dtype = 0, k_cache.dtype
+    if cache_dtype == torch.int8:
         kv_int8 = 1
         if v_cache.dtype != torch.int8 or k_scales is None or v_scales is None:
             raise ValueError(f"{name}: an int8 pool needs int8 k_cache and v_cache and k_scales, v_scales")
@@ -540,35 +534,38 @@ def qk_norm_rope_append(
         for t in (k_scales, v_scales):
             if t.dtype != torch.float32 or tuple(t.shape) != (nb, ch, bs) or not t.is_contiguous():
                 raise ValueError(f"{name}: scales must be contiguous float32 [{nb}, {ch}, {bs}]")
-    elif k_cache.dtype != dtype or v_cache.dtype != dtype:
-        raise RuntimeError(f"{name}: input dtype {dtype} does not match cache dtype {k_cache.dtype}")
-    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != n:
+    elif cache_dtype != dtype or v_cache.dtype != dtype:
+        raise RuntimeError(f"{name}: input dtype {dtype} does not match cache dtype {cache_dtype}")
+    if slot_mapping.shape != (n,):
         raise ValueError(f"{name}: slot_mapping must be [N]={n}, got {tuple(slot_mapping.shape)}")
     if slot_mapping.dtype != torch.int64:
         slot_mapping = slot_mapping.to(torch.int64)
     slot_mapping = slot_mapping.contiguous()
-    hq = q_sn = q_sh = qo_sn = qo_sh = 0
+    q_at = q_out_at = q_sn = q_sh = qo_sn = qo_sh = 0
     if q is None:
         q_out = None
     else:
+        q, q_sn, q_sh = _rows(q)
         if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(-1) != 1:
-            raise ValueError(f"{name}: q_out must be shaped like q, in its dtype, with a contiguous last axis")
-        elif any(st == 0 and size > 1 for st, size in zip(q_out.stride(), q_out.shape)):
-            raise ValueError(f"{name}: q_out must not be an expanded view")
-        hq = q.shape[1]
-        q_sn, q_sh, _ = q.stride()
-        qo_sn, qo_sh, _ = q_out.stride()
-    k_sn, k_sh, _ = k_new.stride()
-    v_sn, v_sh, _ = v_new.stride()
+            q_out = q.new_empty((n, hq, D))
+            qo_sn, qo_sh = hq * D, D
+        else:
+            st = q_out.stride()
+            if q_out.shape != q.shape or q_out.dtype != dtype or st[-1] != 1:
+                raise ValueError(f"{name}: q_out must be shaped like q, in its dtype, with a contiguous last axis")
+            if any(a == 0 and size > 1 for a, size in zip(st, q_out.shape)):
+                raise ValueError(f"{name}: q_out must not be an expanded view")
+            qo_sn, qo_sh = st[0], st[1]
+        q_at, q_out_at = q.data_ptr(), q_out.data_ptr()
+    k_new, k_sn, k_sh = _rows(k_new)
+    v_new, v_sn, v_sh = _rows(v_new)
     _norm_append(index,
-                 q.data_ptr() if hq else 0, k_new.data_ptr(), v_new.data_ptr(), q_out.data_ptr() if hq else 0, 0,
+                 q_at, k_new.data_ptr(), v_new.data_ptr(), q_out_at, 0,
                  k_cache.data_ptr(), v_cache.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), cos.data_ptr(),
                  sin.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
                  n, hq, hkv, D, nb, bs, cos.shape[0],
                  q_sn, q_sh, k_sn, k_sh, v_sn, v_sh, qo_sn, qo_sh, 0, 0, strides[0], strides[1], strides[2], cos.stride(0),
-                 eps, 1 if interleaved else 0, 1 if cos.dtype == torch.float32 else 0, code, kv_int8,
+                 eps, 1 if interleaved else 0, f32, code, kv_int8,
                  k_scales.data_ptr() if kv_int8 else 0, v_scales.data_ptr() if kv_int8 else 0, N.stream_of(index))
     return q_out
 

@@ -155,64 +155,80 @@ _dense = N.Entry("rfx_qk_norm_rope", N.QkNormRopeArgs)
 
 
 def _norm_inputs(name, q, k, q_weight, k_weight, cos, sin, positions, eps):
-    """The checks that the dense form and the append share; returns ``(cos, sin, positions, q_weight, k_weight)``
-    as the kernel takes them. ``q`` may be ``None`` (no query heads)."""
-    shape, dtype = k.shape, k.dtype
-    if len(shape) != 3 or (q is not None and (q.dim() != 3 or q.shape[0] != shape[0] or q.shape[2] != shape[2])):
-        raise ValueError(f"{name}: q must be [N, H_q, D] and k [N, H_kv, D]; "
-                         f"got {None if q is None else tuple(q.shape)} and {tuple(shape)}")
-    n, _, D = shape
+    """The checks that the dense form and the append share; returns ``(n, H_kv, D, H_q, dtype, cos, sin,
+    positions, q_weight, k_weight, table_f32)`` as the kernel takes them. ``q`` may be ``None`` (no query
+    heads). Every attribute is read once: for a decode step this costs more than the kernel."""
+    shape, dtype, hq = k.shape, k.dtype, 0
+    if q is not None:
+        q_shape = q.shape
+        if len(q_shape) != 3 or len(shape) != 3 or q_shape[0] != shape[0] or q_shape[2] != shape[2]:
+            raise ValueError(f"{name}: q must be [N, H_q, D] and k [N, H_kv, D]; got {tuple(q_shape)} and {tuple(shape)}")
+        if q.dtype != dtype:
+            raise RuntimeError(f"{name}: q dtype {q.dtype} differs from k dtype {dtype}")
+        hq = q_shape[1]
+    elif len(shape) != 3:
+        raise ValueError(f"{name}: k must be [N, H_kv, D], got {tuple(shape)}")
+    n, hkv, D = shape
     if D % 2 != 0:
         raise ValueError("head_dim must be even for RoPE")
-    if q is not None and q.dtype != dtype:
-        raise RuntimeError(f"{name}: q dtype {q.dtype} differs from k dtype {dtype}")
     for w in (q_weight, k_weight):
-        if w.dim() != 1 or w.shape[0] != D:
+        if w.shape != (D,):
             raise ValueError(f"{name}: weights must be [{D}], got {tuple(w.shape)}")
         if w.dtype != dtype:
             raise RuntimeError(f"{name}: weight dtype {w.dtype} differs from the activations' {dtype}")
-    if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape:
-        raise ValueError(f"{name}: cos/sin must both be [rows, {D}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    rows = cos.shape
+    if len(rows) != 2 or rows[1] != D or sin.shape != rows:
+        raise ValueError(f"{name}: cos/sin must both be [rows, {D}], got {tuple(rows)} and {tuple(sin.shape)}")
     table = cos.dtype
     if (table != torch.float32 and table != dtype) or sin.dtype != table:
-        cos, sin = cos.to(dtype), sin.to(dtype)
-    if not (cos.is_contiguous() and sin.is_contiguous()) and (cos.stride(1) != 1 or sin.stride() != cos.stride()):
+        cos, sin, table = cos.to(dtype), sin.to(dtype), dtype
+    strides = cos.stride()
+    if strides[1] != 1 or sin.stride() != strides:
         cos, sin = cos.contiguous(), sin.contiguous()
     if positions is not None:
-        if positions.dim() != 1 or positions.shape[0] != n:
+        if positions.shape != (n,):
             raise ValueError(f"{name}: positions must be [N]={n}, got {tuple(positions.shape)}")
         if positions.dtype != torch.int32:
             if positions.dtype == torch.int64:
                 positions = positions.clamp(-1, 2**31 - 1)
             positions = positions.to(torch.int32)
         positions = positions.contiguous()
-    elif n > cos.shape[0]:
-        raise ValueError(f"{name}: {n} tokens without positions need as many table rows, got {cos.shape[0]}")
+    elif n > rows[0]:
+        raise ValueError(f"{name}: {n} tokens without positions need as many table rows, got {rows[0]}")
     if not 0.0 <= eps < 3e38:
         raise ValueError(f"{name}: eps must not be negative, got {eps}")
-    return cos, sin, positions, q_weight.contiguous(), k_weight.contiguous()
+    return (n, hkv, D, hq, dtype, cos, sin, positions, q_weight.contiguous(), k_weight.contiguous(),
+            1 if table == torch.float32 else 0)
+
+
+def _rows(t):
+    """``t`` and its token and head strides, its last axis contiguous (a copy where it is not)."""
+    st = t.stride()
+    if st[-1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, st[0], st[1]
 
 
 def _norm_rope(name, q, k, in_place, q_weight, k_weight, cos, sin, positions, eps, interleaved):
     index = N.same_device(name, k, q, q_weight, k_weight, cos, sin, positions)
-    cos, sin, positions, q_weight, k_weight = _norm_inputs(name, q, k, q_weight, k_weight, cos, sin, positions, eps)
+    n, hkv, D, hq, _, cos, sin, positions, q_weight, k_weight, f32 = _norm_inputs(
+        name, q, k, q_weight, k_weight, cos, sin, positions, eps)
     code = N.dtype_code(k)
+    q, q_sn, q_sh = _rows(q)
+    k, k_sn, k_sh = _rows(k)
     if in_place:
-        q_out, k_out = q, k
+        q_out, k_out, qo_sn, qo_sh, ko_sn, ko_sh = q, k, q_sn, q_sh, k_sn, k_sh
     else:
-        q_out, k_out = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
-    n, hkv, D = k.shape
-    q_sn, q_sh, _ = q.stride()
-    k_sn, k_sh, _ = k.stride()
-    qo_sn, qo_sh, _ = q_out.stride()
-    ko_sn, ko_sh, _ = k_out.stride()
+        q_out, k_out = q.new_empty((n, hq, D)), k.new_empty((n, hkv, D))
+        qo_sn, qo_sh, ko_sn, ko_sh = hq * D, D, hkv * D, D
     _dense(index,
            q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(), 0, 0,
            0, 0 if positions is None else positions.data_ptr(), cos.data_ptr(), sin.data_ptr(),
            q_weight.data_ptr(), k_weight.data_ptr(),
-           n, q.shape[1], hkv, D, 0, 0, cos.shape[0],
+           n, hq, hkv, D, 0, 0, cos.shape[0],
            q_sn, q_sh, k_sn, k_sh, 0, 0, qo_sn, qo_sh, ko_sn, ko_sh, 0, 0, 0, cos.stride(0),
-           eps, 1 if interleaved else 0, 1 if cos.dtype == torch.float32 else 0, code, 0, 0, 0, N.stream_of(index))
+           eps, 1 if interleaved else 0, f32, code, 0, 0, 0, N.stream_of(index))
     return q_out, k_out
 
 
@@ -240,10 +256,6 @@ def qk_norm_rope(
     the tables gives zeros.
     """
     N.check_backend(backend)
-    if q.stride(-1) != 1:
-        q = q.contiguous()
-    if k.stride(-1) != 1:
-        k = k.contiguous()
     return _norm_rope("qk_norm_rope", q, k, False, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 

@@ -248,3 +248,29 @@ def test_stream_and_graph(native):
     torch.cuda.synchronize()
     want_q, want_k = qk_norm_rope(q, k, wq, wk, cos, sin, positions=pos)
     assert torch.equal(q_out, want_q) and torch.equal(kc[slots // 16, :, slots % 16], want_k)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_decode_step_with_norm_int8(native, interleaved):
+    """The same step on an int8 pool equals the append with norm and the decode kernel's int8 form."""
+    B, bs, nb = 4, 16, 40
+    cos, sin = _tables(300, 128, interleaved, torch.float32)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    q, k, v, wq, wk = _inputs(B, 8, 2, 128, torch.bfloat16, 4)
+    pools = [int8_pool(nb, 2, bs, 128, DEV) for _ in range(2)]
+    for kc, vc, ks, vs in pools:
+        g.manual_seed(3)
+        kc.random_(-127, 128, generator=g); vc.random_(-127, 128, generator=g)
+        ks.uniform_(0.01, 0.02, generator=g); vs.uniform_(0.01, 0.02, generator=g)
+    table = torch.randperm(nb, device=DEV, generator=g)[:B * 10].view(B, 10)
+    lens = torch.tensor([1, 17, 64, 160], dtype=torch.int32, device=DEV)
+    pos = lens - 1
+    slots = table.gather(1, (pos // bs).long()[:, None])[:, 0] * bs + pos % bs
+    (k1, v1, ks1, vs1), (k2, v2, ks2, vs2) = pools
+    got = paged_decode_step(q, k, v, k1, v1, table, lens, slots, pos, cos, sin, interleaved=interleaved, k_scales=ks1,
+                            v_scales=vs1, q_norm_weight=wq, k_norm_weight=wk, norm_eps=1e-5)
+    qr = qk_norm_rope_append(q, k, v, k2, v2, slots, pos, cos, sin, wq, wk, eps=1e-5, interleaved=interleaved, k_scales=ks2,
+                             v_scales=vs2)
+    want = paged_decode(qr, k2, v2, table, lens, k_scales=ks2, v_scales=vs2)
+    for a, b in ((got, want), (k1, k2), (v1, v2), (ks1, ks2), (vs1, vs2)):
+        assert torch.equal(a, b)
