@@ -43,8 +43,8 @@ using u64 = unsigned long long;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCap = 2048;     // logits that one CTA ranks
-constexpr int kPairs = 128;     // a list up to here is ranked by comparing all pairs, a longer one sorted (300: 10 and 4 us)
-constexpr int kPairsCut = 256;  // the same for the bin with a border (200: 4 and 7 us)
+constexpr int kPairs = 128;     // a list up to here is ranked by comparing all pairs, a longer one sorted (300: 10 and 4 us) or narrowed
+                                // down (32 x 50257 bf16, top-p, some 130 to 260 logits in the border's bin: 25.5 us; with 256 here 26.5, 0: 26.9)
 constexpr int kBins = 2048;   // more than 32 * (S + 2), the steps to a weight of zero
 constexpr int kMaxCluster = 8;
 constexpr int kGroups = 2 * kThreads;     // groups whose maxima bound the k-th largest logit
@@ -75,11 +75,10 @@ struct __align__(16) Shared {
     union {
         struct { uint32_t lo[kBins], hi[kBins]; } hist;
         u64 weight[kCap];       // of the sorted list
-        Entry pair[kPairsCut];  // of the list where all pairs are compared
+        Entry pair[kPairs];  // of the list where all pairs are compared
         uint32_t group[kGroups];
     };
     u64 part[kWarps];
-    u64 ends[2][kWarps];
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
     u64 shares[2][kMaxCluster][kMaxCluster];  // [top-k, top-p][CTA][share of the bins]: what that CTA's logits add to it
     u64 found[3];              // what one CTA tells all: a bin and the sum before it, a cut
@@ -557,7 +556,7 @@ template <typename T> struct Row {
         if (n <= kCap) {
             u64 key = 0;
             if (rank == 0) {
-                if (n <= kPairsCut) {
+                if (n <= kPairs) {
                     rank_pairs<MASS>(n, [&](u64 e, int, u64 before, u64 m) {
                         before += above;
                         if (before < target && before + m >= target) s.found[0] = e;
@@ -565,7 +564,7 @@ template <typename T> struct Row {
                     __syncthreads();
                     key = s.found[0];
                 } else {
-                    key = border<MASS>(n, above, target);
+                    key = border<MASS>(n, above, target, dense_of((u64)key_of(from) << 32), dense_of((u64)key_of(to) << 32 | 0xffffffffu));
                 }
             }
             key = tell(key);
@@ -683,13 +682,19 @@ template <typename T> struct Row {
         }
     }
 
+    // An entry's rank as a number without gaps: value (without the bits that T does not have), then index.
+    __device__ __forceinline__ u64 dense_of(u64 entry) const {
+        const int bits = 32 - __clz(vocab - 1);  // of an index
+        constexpr int kEmpty = std::is_same_v<T, __nv_bfloat16> ? 16 : std::is_same_v<T, __half> ? 13 : 0;
+        return (u64)((uint32_t)(entry >> 32) >> kEmpty) << bits | ((uint32_t)entry & ((1u << bits) - 1));
+    }
     // The entry of list[0, n) at which the sum of masses (or 1 each) over falling entries, with `above` before the first, first
-    // reaches the target. A histogram over the ten highest bits in which two entries differ, again and again over the
-    // bin with the border, until one entry is left: two or three rounds of 2 us, however many logits are equal (then their
-    // indexes differ).
-    template <bool MASS> __device__ __forceinline__ u64 border(int n, u64 above, u64 target) {
+    // reaches the target; all dense numbers lie in [low, high]. A histogram of 1024 steps over [low, high], again over the
+    // step with the border while that holds more than a warp can rank: one round for as good as every row, for equal
+    // logits too (then the steps part their indexes).
+    template <bool MASS> __device__ __forceinline__ u64 border(int n, u64 above, u64 target, u64 low, u64 high) {
         constexpr int PER = kCap / kThreads;
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int lane = threadIdx.x & 31;
         u64 e[PER], m[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
@@ -698,33 +703,19 @@ template <typename T> struct Row {
             m[j] = i < n ? (MASS ? mass((uint32_t)(e[j] >> 32)) : 1) : 0;
         }
         for (;;) {
-            u64 high = 0, low = ~0ull;
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                high = max(high, e[j]);
-                if (e[j]) low = min(low, e[j]);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
-                low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-            }
+            const int shift = max(0, 54 - __clzll((long long)(high - low | 1)));
             __syncthreads();
-            if (lane == 0) { s.ends[0][warp] = high; s.ends[1][warp] = low; }
             reinterpret_cast<uint2*>(s.hist.lo)[threadIdx.x] = reinterpret_cast<uint2*>(s.hist.hi)[threadIdx.x] = make_uint2(0, 0);
+            if (threadIdx.x == 0) s.n = 0;
             __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) { high = max(high, s.ends[0][w]); low = min(low, s.ends[1][w]); }
-            if (high == low) return high;
-            const int first = 63 - __clzll((long long)(high ^ low)), shift = max(0, first - 9);
-            const u64 base = first == 63 ? 0 : high >> (first + 1) << (first + 1);
+            int at[PER];
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
                 if (!e[j]) continue;
-                const int b = 1023 - (int)((e[j] - base) >> shift);  // the largest in front
-                const uint32_t add = (uint32_t)m[j], old = atomicAdd(&s.hist.lo[b], add);
+                at[j] = (int)((high - dense_of(e[j])) >> shift);  // the largest in front
+                const uint32_t add = (uint32_t)m[j], old = atomicAdd(&s.hist.lo[at[j]], add);
                 const uint32_t up = (uint32_t)(m[j] >> 32) + (old + add < old ? 1u : 0u);
-                if (up) atomicAdd(&s.hist.hi[b], up);
+                if (up) atomicAdd(&s.hist.hi[at[j]], up);
             }
             __syncthreads();
             const uint2 l = reinterpret_cast<const uint2*>(s.hist.lo)[threadIdx.x], h = reinterpret_cast<const uint2*>(s.hist.hi)[threadIdx.x];
@@ -737,15 +728,33 @@ template <typename T> struct Row {
                 s.found[1] = before + (second ? m0 : 0);
             }
             __syncthreads();
-            const int bin = (int)s.found[0];
+            const int step = (int)s.found[0];
             above = s.found[1];
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (e[j] && 1023 - (int)((e[j] - base) >> shift) != bin) e[j] = 0;
+            for (int j = 0; j < PER; ++j) {
+                if (!e[j]) continue;
+                if (at[j] != step) { e[j] = 0; continue; }
+                const int x = atomicAdd(&s.n, 1);
+                if (x < 32) s.pair[x] = Entry{e[j], m[j]};
+            }
+            __syncthreads();
+            const int left = s.n;
+            if (left <= 32 || shift == 0) {  // (a step of one dense number holds one entry)
+                const Entry mine = s.pair[lane < left ? lane : 0];
+                u64 sum = above;
+                for (int j = 0; j < left; ++j) {
+                    const Entry o = s.pair[j];
+                    if (o.key > mine.key) sum += o.mass;
+                }
+                const uint32_t hit = __ballot_sync(0xffffffffu, lane < left && sum < target && sum + mine.mass >= target);
+                return __shfl_sync(0xffffffffu, mine.key, __ffs(hit) - 1);
+            }
+            high -= (u64)step << shift;
+            low = max(low, high - ((1ull << shift) - 1));
         }
     }
 
-    // f(entry, its place, the sum before it, its own mass or 1) for list[0, n), n <= kPairsCut, all in falling order,
+    // f(entry, its place, the sum before it, its own mass or 1) for list[0, n), n <= kPairs, all in falling order,
     // without sorting: a thread compares its entry with every other.
     template <bool MASS, typename F> __device__ __forceinline__ void rank_pairs(int n, F f) {
         const int i = threadIdx.x;

@@ -85,6 +85,20 @@ def test_equal_logits(native, V):
     _same(x, u, temperature=0.0)
 
 
+@pytest.mark.parametrize("offset", [0.0, -40.0, 3e4])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V,width", [(1500, 0.05), (1999, 1e-3), (4097, 0.1), (50257, 0.5)])
+def test_crowded_borders(native, V, width, dtype, offset):
+    """Rows so narrow that hundreds of logits, distinct and equal ones, share the border's bin."""
+    g = torch.Generator().manual_seed(V)
+    x = (offset + width * torch.randn(4, V, generator=g)).to(dtype)
+    x[3, ::7] = offset
+    u = torch.rand(4, generator=g)
+    for kw in (dict(top_p=0.9), dict(top_p=0.37), dict(top_k=V - 600), dict(top_k=V // 2, top_p=0.6),
+               dict(top_p=0.5, temperature=40.0), dict(top_k=V - 700, temperature=1e30), dict(top_p=0.8, temperature=1e-3)):
+        _same(x, u, **kw)
+
+
 def test_masks_infinities_and_nan(native):
     V = 6000
     x, _ = _rows(10, V, torch.float32, 9)
