@@ -54,6 +54,7 @@ constexpr size_t kStageTwo = 72 * 1024;   // slice that lets two CTAs share an S
 constexpr size_t kStageMax = 180 * 1024;  // largest slice kept in shared memory
 constexpr float kLowest = -3.402823466e38f;
 
+enum { kAllRows = 0, kListRows = 1, kOtherRows = 2 };
 struct SampleParams {
     const void* logits;
     const float *u, *temperature, *top_p, *min_p;
@@ -66,6 +67,7 @@ struct SampleParams {
     int shift;         // S: weights are multiples of 2^-S
     double power[32];  // 2^(S + i/32), with i * 2^15 taken off the upper word
     int staged;        // general rows keep their slice in shared memory
+    int rows;          // which rows this launch takes
 };
 
 struct __align__(16) Entry { u64 key, mass; };  // key: the logit's ordered bits, then ~index
@@ -1049,6 +1051,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     int64_t* token = P.tokens + b;
     const bool greedy = !(temperature > 0.f), by_list = !greedy && k < P.vocab && k <= kListK;
 
+    if (P.rows != kAllRows && by_list != (P.rows == kListRows)) {  // the other launch's
+        cluster.barrier_wait(std::move(started));
+        return;
+    }
+
     const double t = fmax((double)temperature, 1e-20);
     r.scale = fmax(32.0 * 1.4426950408889634 / t, 1e-300);  // at T = inf every finite logit weighs 1
     r.cut_index = 0x7fffffff;
@@ -1097,21 +1104,25 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
 
-    // CTAs of a row: as many as give every SM one while a CTA keeps 8 logits or more a thread (256 x 131072 fp32, top-k: one a
-    // row 41.7 us, two 57.6). Settings given row by row give rows of unequal work; then twice as many, if one is not
-    // enough anyway (64 x 131072 bf16: mixed rows 40.2 us with eight a row, 48.1 with four; rows with top-k alone 21.0 and 14.8).
-    const bool unequal = a->temperature || a->top_k || a->top_p || a->min_p;
-    int C = 1;
+    // CTAs of a row. List rows: as many as give every SM one while a CTA keeps 8 logits or more a thread (256 x 131072 fp32: one
+    // a row 34 us, two 58). General rows, bound by instructions, also fill both places of an SM while a CTA keeps 64
+    // (256 x 131072 fp32, top-p: 215 us with one a row, 196 with two, 206 with four; 512 x 50257: 160, 169, 201). Settings given
+    // row by row give rows of unequal work: twice as many (64 x 131072 bf16: mixed rows 38 us with eight a row, 46 with four,
+    // lists alone 21.7 and 15; 256 x 131072 fp32 mixed: 148 with two, 127 with four).
+    const bool unequal = a->temperature || a->top_k || a->top_p || a->min_p, all_lists = !a->top_k && a->top_k_all > 0 && a->top_k_all <= kListK;
     auto slice_of = [&](int c) { return round_up<int64_t>(ceil_div<int64_t>(a->vocab, c), 8); };
-    while (C < kMaxCluster && a->batch < sm_count() && a->batch * C < (unequal ? 2 : 1) * sm_count() && slice_of(C) > 8 * kThreads) C *= 2;
-    const int64_t slice = slice_of(C);
-    const size_t bytes = round_up<size_t>((size_t)(slice + 8) * e, 16);
-    const bool staged = bytes <= (a->batch * C > sm_count() ? kStageTwo : kStageMax);
+    auto grow = [&](int c, int64_t ctas, int64_t logits) {
+        while (c < kMaxCluster && a->batch * c < ctas && slice_of(c) > logits) c *= 2;
+        return c;
+    };
+    const int64_t sms = sm_count();
+    const int C_lists = grow(1, sms, 8 * kThreads);
+    const int C_others = grow(grow(1, unequal && a->batch < sms ? 2 * sms : sms, 8 * kThreads), (unequal ? 4 : 2) * sms, 64 * kThreads);
     SampleParams P = {};
     P.logits = a->logits; P.u = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p;
     P.top_k = a->top_k; P.tokens = a->tokens; P.row_stride = a->row_stride;
     P.temperature0 = a->temperature_all; P.top_p0 = a->top_p_all; P.min_p0 = a->min_p_all; P.top_k0 = a->top_k_all;
-    P.vocab = (int)a->vocab; P.slice = (int)slice; P.staged = staged ? 1 : 0;
+    P.vocab = (int)a->vocab;
     int log2v = 0;
     while ((1ll << log2v) < a->vocab) ++log2v;
     P.shift = 62 - log2v < 50 ? 62 - log2v : 50;
@@ -1123,33 +1134,44 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
         memcpy(&P.power[i], &bits, 8);
     }
 
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a->batch * C));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = staged ? bytes : 0;
-    cfg.stream = as_stream(a->stream);
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)C;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
     cudaError_t le = cudaSuccess;
-    auto launch = [&](auto kern, PerDeviceOnce& once) {
+    auto launch = [&](auto kern, PerDeviceOnce& once, int C, int rows) {
+        P.slice = (int)slice_of(C);
+        P.rows = rows;
+        const size_t bytes = round_up<size_t>((size_t)(P.slice + 8) * e, 16);
+        P.staged = rows != kListRows && bytes <= (a->batch * C > sm_count() ? kStageTwo : kStageMax) ? 1 : 0;
         int dev = 0;
         cudaGetDevice(&dev);
-        if (staged && !once.done(dev)) {
+        if (P.staged && !once.done(dev)) {
             le = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kStageMax);
             if (le != cudaSuccess) return;
             once.mark(dev);
         }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(a->batch * C));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = P.staged ? bytes : 0;
+        cfg.stream = as_stream(a->stream);
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = (unsigned)C;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
         le = cudaLaunchKernelEx(&cfg, kern, P);
     };
     RFX_DISPATCH_DTYPE(a->dtype, T, {
         static PerDeviceOnce once;
-        launch(sample_kernel<T>, once);
+        // Where list rows want one CTA and the others several, each kind has a launch of its own (256 x 131072 fp32, lists
+        // alone: 39 us, in one launch of one CTA a row 34; mixed: 127 and 179).
+        if (a->top_k && C_lists == 1 && C_others > 1) {
+            launch(sample_kernel<T>, once, C_lists, kListRows);
+            if (le == cudaSuccess) launch(sample_kernel<T>, once, C_others, kOtherRows);
+        } else {
+            launch(sample_kernel<T>, once, all_lists ? C_lists : C_others, kAllRows);
+        }
     });
     if (le != cudaSuccess) { cudaGetLastError(); return fail(RFX_CUDA_ERROR, "%s: %s", name, cudaGetErrorString(le)); }
     return check_launch(name);

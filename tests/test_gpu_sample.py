@@ -71,6 +71,17 @@ def test_settings_per_row_and_batch_sizes(native, dtype):
         assert sample_tokens(x[:n].to(DEV), u[:n].to(DEV), **part).tolist() == whole[:n]
 
 
+@pytest.mark.parametrize("B,V", [(100, 9001), (200, 70001)])
+def test_list_rows_beside_others(native, B, V):
+    """Rows with a small top-k in a batch with others, in one launch and in two; among them some whose thousands
+    of equal logits overflow the list."""
+    x, u = _rows(B, V, torch.bfloat16, 6)
+    x[::5] = torch.round(x[::5])
+    x[7] = -math.inf
+    top_k = torch.tensor([30, 0, 511, 1])[torch.arange(B) % 4].to(torch.int32)
+    _same(x, u, top_k=top_k, top_p=torch.tensor([0.9, 1.0])[torch.arange(B) % 2])
+
+
 @pytest.mark.parametrize("V", [64, 5000, 40000])
 def test_equal_logits(native, V):
     """All logits equal: every border is a whole number of tokens, hit exactly; far more ties than a list takes."""
