@@ -52,6 +52,7 @@ constexpr int kListK = kGroups / 2;       // with k near kGroups the bound sinks
 constexpr int kBatch = 4;                 // 16-byte chunks a thread has under way
 constexpr size_t kStageTwo = 72 * 1024;   // slice that lets two CTAs share an SM
 constexpr size_t kStageMax = 180 * 1024;  // largest slice kept in shared memory
+constexpr int kParts = 8;                 // of a warp's range in the draw
 constexpr float kLowest = -3.402823466e38f;
 
 enum { kAllRows = 0, kListRows = 1, kOtherRows = 2 };
@@ -265,6 +266,7 @@ template <typename T> struct Row {
     float zero_below;     // logits below weigh less than 2^-S-1: nothing
     float cut_value;      // kept: v > cut_value, or v == cut_value and index <= cut_index
     int cut_index;
+    float cut_next;       // the value above cut_value
 
     __device__ __forceinline__ void set_top(float v) {
         top = v;
@@ -310,6 +312,17 @@ template <typename T> struct Row {
             if (j < nvec && (j < first || j > last)) to[x] = load_edge(j);
         }
     }
+    // The same from shared memory where the slice is there.
+    __device__ __forceinline__ void fetch_any(Chunk<T> (&to)[kBatch], int j0) const {
+        if (staged) {
+#pragma unroll
+            for (int x = 0; x < kBatch; ++x) to[x].raw = reinterpret_cast<const uint4*>(stage)[min(j0 + x * kThreads, nvec - 1)];
+        } else if (inside(j0 - threadIdx.x)) {
+            fetch<true>(to, j0);
+        } else {
+            fetch<false>(to, j0);
+        }
+    }
     __device__ __forceinline__ Chunk<T> load(int j) const {
         if (!staged) return load_global(j);
         Chunk<T> c;
@@ -345,7 +358,7 @@ template <typename T> struct Row {
     // A pass over weights is bound by the integer and compare instructions (half rate) and the nine 64-bit operations. So
     // n is rounded in 64 bits too, the float is widened by the conversion unit, and the table's entries have their
     // place in the table taken off the exponent's field: n * 2^15 added to the upper word is the whole shift.
-    __device__ __forceinline__ u64 mass_of(float v, int& bin) const {
+    __device__ __forceinline__ double mass_of(float v, int& bin) const {
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
         const double d = (double)fminf(v, -kLowest) - top_wide;
         const double t = fma(d, scale, kMagic);
@@ -357,17 +370,29 @@ template <typename T> struct Row {
         p = fma(p, f, kTerm[0]);
         p = fma(p, f, 1.0);
         const double w = s.power[n & 31];
-        const double sum = fma(p, __hiloint2double(__double2hiint(w) + n * 32768, __double2loint(w)), 4503599627370496.0);
-        return (u64)__double_as_longlong(sum) & 0xfffffffffffffull;
+        return fma(p, __hiloint2double(__double2hiint(w) + n * 32768, __double2loint(w)), kWhole);
     }
+    static constexpr double kWhole = 4503599627370496.0;  // 2^52: a mass, added to it, is the low 52 bits
+    __device__ __forceinline__ static u64 low52(double m) { return (u64)__double_as_longlong(m) & 0xfffffffffffffull; }
     __device__ __forceinline__ int bin_of(float v) const {
         return -__double2loint(fma((double)fminf(v, -kLowest) - top_wide, scale, 6755399441055744.0));
     }
     __device__ __forceinline__ u64 mass(uint32_t key) const {
         int unused;
-        return value_of(key) >= zero_below ? mass_of(value_of(key), unused) : 0;
+        return value_of(key) >= zero_below ? low52(mass_of(value_of(key), unused)) : 0;
     }
     __device__ __forceinline__ bool kept(float v, int i) const { return v >= cut_value && (v > cut_value || i <= cut_index); }
+    // The logits of the chunk from index i0 on that are kept are those from the returned value on: the cut, or the next value above
+    // it behind the last index that stays. The one chunk with that index inside loses the others at the cut.
+    __device__ __forceinline__ float cut_of(Chunk<T>& c, int i0) const {
+        if (i0 + N - 1 > cut_index) {
+            if (i0 > cut_index) return cut_next;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (!kept(c.raw_at(e), i0 + e)) c.v[e] = Num<T>::from_f(-INFINITY);
+        }
+        return cut_value;
+    }
     __device__ __forceinline__ static u64 warp_total(u64 v) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -455,26 +480,26 @@ template <typename T> struct Row {
     template <bool MASS> __device__ __forceinline__ void cut(int k, float p) {
         reinterpret_cast<uint4*>(s.hist.lo)[threadIdx.x] = reinterpret_cast<uint4*>(s.hist.hi)[threadIdx.x] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        each_chunk([&](const Chunk<T>& c, int i0) {
-            if (!(c.most() >= cut_value)) return;
+        each_chunk([&](Chunk<T> c, int i0) {
+            const float from = cut_of(c, i0);
+            if (!(c.most() >= from)) return;
             int bin[N];
-            u64 w[N];
+            double w[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 if (MASS) w[e] = mass_of(c.raw_at(e), bin[e]);
                 else bin[e] = bin_of(c.raw_at(e));
             }
+            uint32_t old[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const int b = bin[e];
-                if (!kept(c.raw_at(e), i0 + e)) continue;
-                if (MASS) {  // 64 bits as two words: the one that overflows the low word carries
-                    const uint32_t low = (uint32_t)w[e], old = atomicAdd(&s.hist.lo[b], low);
-                    const uint32_t high = (uint32_t)(w[e] >> 32) + (old + low < old ? 1u : 0u);
-                    if (high) atomicAdd(&s.hist.hi[b], high);
-                } else {
-                    atomicAdd(&s.hist.lo[b], 1u);
-                }
+            for (int e = 0; e < N; ++e)
+                old[e] = c.raw_at(e) >= from ? atomicAdd(&s.hist.lo[bin[e]], MASS ? (uint32_t)__double2loint(w[e]) : 1u) : 0u;
+            if (!MASS) return;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {  // 64 bits as two words: the one that overflows the low word carries
+                const uint32_t low = (uint32_t)__double2loint(w[e]);
+                const uint32_t high = ((uint32_t)__double2hiint(w[e]) & 0xfffffu) + (old[e] + low < low ? 1u : 0u);
+                if (c.raw_at(e) >= from && high) atomicAdd(&s.hist.hi[bin[e]], high);
             }
         });
         // The bins are cut into one share per CTA. Everyone tells everyone what its own logits add to each share, so after one
@@ -547,13 +572,20 @@ template <typename T> struct Row {
         const bool windowed = top < INFINITY && width < 1e30f && slack < 1e30f;
         const float from = windowed ? top - ((float)bin + 0.5f) * width - slack : kLowest;
         const float to = windowed ? top - ((float)bin - 0.5f) * width + slack : INFINITY;
-        each_chunk([&](const Chunk<T>& c, int i0) {
+        for (int j0 = threadIdx.x; j0 < nvec; j0 += kBatch * kThreads) {
+            Chunk<T> c[kBatch];
+            fetch_any(c, j0);
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                const float v = c.raw_at(e);
-                if (v >= from && v <= to && kept(v, i0 + e) && bin_of(v) == bin) put(v, i0 + e);
+            for (int x = 0; x < kBatch; ++x) {
+                if (j0 + x * kThreads >= nvec || !(c[x].most() >= from)) continue;
+                const int i0 = base + (j0 + x * kThreads) * N;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float v = c[x].raw_at(e);
+                    if (v >= from && v <= to && kept(v, i0 + e) && bin_of(v) == bin) put(v, i0 + e);
+                }
             }
-        });
+        }
         const int n = collect();
         if (n <= kCap) {
             u64 key = 0;
@@ -571,6 +603,7 @@ template <typename T> struct Row {
             }
             key = tell(key);
             cut_value = value_of((uint32_t)(key >> 32));
+            cut_next = value_of((uint32_t)(key >> 32) + 1u);
             cut_index = (int)(0xffffffffu - (uint32_t)key);
             return;
         }
@@ -599,6 +632,7 @@ template <typename T> struct Row {
             if (cluster_sum(t) < ties) index = to;
         }
         cut_value = value_of(key);
+        cut_next = value_of(key + 1u);
         cut_index = index + 1;
     }
 
@@ -622,10 +656,12 @@ template <typename T> struct Row {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
         const int per = (nvec + kWarps - 1) / kWarps, from = warp * per, to = min(nvec, from + per);
         const u64 least = least_of(min_p);
+        const double least_whole = kWhole + (double)least;
         // the masses of a chunk's logits that stay; their sum
-        auto masses = [&](const Chunk<T>& c, int j, u64 (&m)[N]) {
+        auto masses = [&](Chunk<T> c, int j, u64 (&m)[N]) {
             u64 sum = 0;
-            if (!(c.most() >= cut_value)) {
+            const float cut = cut_of(c, base + j * N);
+            if (!(c.most() >= cut)) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) m[e] = 0;
                 return sum;
@@ -633,18 +669,28 @@ template <typename T> struct Row {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 int unused;
-                const u64 w = mass_of(c.raw_at(e), unused);
-                m[e] = kept(c.raw_at(e), base + j * N + e) && w >= least ? w : 0;
+                const double w = mass_of(c.raw_at(e), unused);
+                m[e] = c.raw_at(e) >= cut && w >= least_whole ? low52(w) : 0;
                 sum += m[e];
             }
             return sum;
         };
-        u64 sum = 0;
-        chunks(from + lane, to, 32, [&](const Chunk<T>& c, int j) {
-            u64 m[N];
-            sum += masses(c, j, m);
-        });
-        const u64 all = warp_total(sum);
+        // The lanes' sums over each part of the warp's range stay in shared memory: the warp with the token looks into one
+        // part alone (through a whole range of 131072 / 16 logits it took up to 27 us).
+        static_assert(kParts == 8 && 4 * kThreads == kCap, "four parts in the list's place, four in the weights'");
+        const int span = 32 * max(4, (per + 32 * kParts - 1) / (32 * kParts));
+        auto part_sum = [&](int part) -> u64& { return (part < 4 ? s.list : s.weight)[(part & 3) * kThreads + threadIdx.x]; };
+        u64 all = 0;
+        for (int start = from, part = 0; start < to; start += span, ++part) {
+            u64 sum = 0;
+            chunks(start + lane, min(to, start + span), 32, [&](const Chunk<T>& c, int j) {
+                u64 m[N];
+                sum += masses(c, j, m);
+            });
+            part_sum(part) = sum;
+            all += sum;
+        }
+        all = warp_total(all);
         __syncthreads();
         if (lane == 0) s.part[warp] = all;
         __syncthreads();
@@ -658,7 +704,13 @@ template <typename T> struct Row {
         before += warp_total(lane < rank ? each_cta : 0);
         const u64 target = drawn(u, total);
         if (target < before || target >= before + all) return;  // whole warps
-        for (int j0 = from; j0 < to; j0 += 32) {
+        int start = from;
+        for (int part = 0; start + span < to; start += span, ++part) {
+            const u64 sum = warp_total(part_sum(part));
+            if (target < before + sum) break;
+            before += sum;
+        }
+        for (int j0 = start; j0 < to; j0 += 32) {
             u64 m[N], own = 0;
             const int j = j0 + lane;
 #pragma unroll
@@ -1104,20 +1156,23 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     int st = check_device();
     if (st != RFX_SUCCESS) return st;
 
-    // CTAs of a row. List rows: as many as give every SM one while a CTA keeps 8 logits or more a thread (256 x 131072 fp32: one
-    // a row 34 us, two 58). General rows, bound by instructions, also fill both places of an SM while a CTA keeps 64
-    // (256 x 131072 fp32, top-p: 215 us with one a row, 196 with two, 206 with four; 512 x 50257: 160, 169, 201). Settings given
-    // row by row give rows of unequal work: twice as many (64 x 131072 bf16: mixed rows 38 us with eight a row, 46 with four,
-    // lists alone 21.7 and 15; 256 x 131072 fp32 mixed: 148 with two, 127 with four).
+    // CTAs of a row. List rows: as many as leave no more than one SM in six without any, at most one an SM while a CTA keeps fewer
+    // than 64 logits a thread, and 8 of those (32 x 50257 bf16: 10 us with four a row, 15.6 with eight; 64 x 131072: 13.3
+    // with two, 15.5 with four; 120 x 131072 fp32: 27.7 with one, 23.2 with two; 256 x 131072: 34 and 44).
+    // General rows, bound by instructions, give every SM one, and fill both its places while a CTA keeps 64 logits a thread (64 x 131072
+    // bf16, top-p: 58 us with two a row, 51 with four, 62 with eight; 256 x 131072 fp32: 193 with one, 182 with two, 198 with
+    // four; 512 x 50257: 149, 166, 198). Settings given row by row give rows of unequal work: twice as many (64 x 131072 bf16
+    // mixed: 44 us with four, 39 with eight; 256 x 131072 fp32: 166, 110, 105 with one, two, four).
     const bool unequal = a->temperature || a->top_k || a->top_p || a->min_p, all_lists = !a->top_k && a->top_k_all > 0 && a->top_k_all <= kListK;
+    const int64_t sms = sm_count();
+    constexpr int64_t kFew = 8 * kThreads, kMany = 64 * kThreads;
     auto slice_of = [&](int c) { return round_up<int64_t>(ceil_div<int64_t>(a->vocab, c), 8); };
     auto grow = [&](int c, int64_t ctas, int64_t logits) {
         while (c < kMaxCluster && a->batch * c < ctas && slice_of(c) > logits) c *= 2;
         return c;
     };
-    const int64_t sms = sm_count();
-    const int C_lists = grow(1, sms, 8 * kThreads);
-    const int C_others = grow(grow(1, unequal && a->batch < sms ? 2 * sms : sms, 8 * kThreads), (unequal ? 4 : 2) * sms, 64 * kThreads);
+    const int C_lists = grow(grow(1, sms / 2 + 1, kFew), sms * 5 / 6, kMany);
+    const int C_others = grow(grow(1, unequal && a->batch < sms ? 2 * sms : sms, kFew), (unequal ? 4 : 2) * sms, kMany);
     SampleParams P = {};
     P.logits = a->logits; P.u = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p;
     P.top_k = a->top_k; P.tokens = a->tokens; P.row_stride = a->row_stride;
@@ -1164,9 +1219,10 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     };
     RFX_DISPATCH_DTYPE(a->dtype, T, {
         static PerDeviceOnce once;
-        // Where list rows want one CTA and the others several, each kind has a launch of its own (256 x 131072 fp32, lists
-        // alone: 39 us, in one launch of one CTA a row 34; mixed: 127 and 179).
-        if (a->top_k && C_lists == 1 && C_others > 1) {
+        // Where top-k is given row by row, in batches that fill the GPU with one CTA a row, list rows want one CTA and the others
+        // several: a launch for each kind (256 x 131072 fp32, lists alone: 39 us, in one launch of one CTA a row 34, of
+        // four 60; mixed: 122, 166 and 105).
+        if (a->top_k && a->batch >= sms && C_others > 1) {
             launch(sample_kernel<T>, once, C_lists, kListRows);
             if (le == cudaSuccess) launch(sample_kernel<T>, once, C_others, kOtherRows);
         } else {
