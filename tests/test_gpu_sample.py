@@ -180,6 +180,15 @@ def test_distribution(native):
     assert (got - p * n).abs().max() <= 1
 
 
+@pytest.mark.parametrize("B,V,dtype", [(300, 60000, torch.float32), (300, 60001, torch.bfloat16), (64, 200003, torch.float16)])
+def test_draws_along_a_row(native, B, V, dtype):
+    """Evenly spaced numbers on one flat row: the token lies in every stretch of it, of every CTA and warp."""
+    x, _ = _rows(1, V, dtype, 21, "flat")
+    u = (torch.arange(B) + 0.25) / B
+    for kw in (dict(), dict(top_p=0.9, min_p=1e-4)):
+        _same(x.expand(B, V), u, x_dev=x.to(DEV).expand(B, V), **kw)
+
+
 def test_refusals(native):
     x, u = torch.zeros(2, 8, device=DEV), torch.zeros(2, device=DEV)
     for bad in (lambda: sample_tokens(x[0], u), lambda: sample_tokens(x, u[:1]), lambda: sample_tokens(x[:, :0], u),
