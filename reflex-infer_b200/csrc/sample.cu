@@ -84,7 +84,7 @@ struct __align__(16) Shared {
     u64 part[kWarps];
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
     u64 shares[2][kMaxCluster][kMaxCluster];  // [top-k, top-p][CTA][share of the bins]: what that CTA's logits add to it
-    u64 found[3];              // what one CTA tells all: a bin and the sum before it, a cut
+    u64 found[3];              // a bin and the sum before it; what one CTA tells all, a cut
     double power[32];          // as in SampleParams
     uint32_t picked[3];        // of select(): the bound, the largest key, n before it
     int n;                     // entries that want to be in `list`
@@ -503,7 +503,8 @@ template <typename T> struct Row {
             }
         });
         // The bins are cut into one share per CTA. Everyone tells everyone what its own logits add to each share, so after one
-        // barrier all know in whose share the border lies, and that CTA alone adds up its share's bins over the cluster.
+        // barrier all know in whose share the border lies, and add up that share's bins over the cluster, each for itself (one CTA for
+        // all would take another cluster barrier). The histograms stay as they are until the exchange in collect().
         __syncthreads();
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = kBins / ranks;
         {
@@ -531,38 +532,36 @@ template <typename T> struct Row {
         u64 total = warp_total(in_share);
         if (!MASS && total <= (u64)k) return;  // the border lies behind the last logit that weighs anything
         const u64 target = MASS ? target_of(p, total) : (u64)k;
-        u64 before = warp_total(lane < rank ? in_share : 0);
-        const u64 mine = __shfl_sync(0xffffffffu, in_share, rank);
-        if (before < target && before + mine >= target) {  // all threads of one CTA
-            const int per = max(1, share / kThreads), first = (int)threadIdx.x * per;
-            u64 m[kBins / kThreads], sum = 0, unused;
+        u64 upto = in_share;
 #pragma unroll
-            for (int j = 0; j < kBins / kThreads; ++j) {
-                m[j] = 0;
-                if (j >= per || first >= share) continue;
-                const int b = rank * share + first + j;
-#pragma unroll
-                for (int r = 0; r < kMaxCluster; ++r) {  // all reads under way together
-                    if (r >= ranks) continue;
-                    m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
-                    if (MASS) m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
-                }
-                sum += m[j];
-            }
-            before += block_scan(sum, unused);
-#pragma unroll
-            for (int j = 0; j < kBins / kThreads; ++j) {
-                if (before < target && before + m[j] >= target) {
-                    for (int r = 0; r < ranks; ++r) {
-                        u64* f = cg::this_cluster().map_shared_rank(s.found, r);
-                        f[0] = (u64)(rank * share + first + j);
-                        f[1] = before;
-                    }
-                }
-                before += m[j];
-            }
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
         }
-        cg::this_cluster().sync();
+        const int of = __ffs(__ballot_sync(0xffffffffu, upto >= target)) - 1;
+        u64 before = __shfl_sync(0xffffffffu, upto - in_share, of);
+        const int per = max(1, share / kThreads), first = (int)threadIdx.x * per;
+        u64 m[kBins / kThreads], sum = 0, unused;
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            m[j] = 0;
+            if (j >= per || first >= share) continue;
+            const int b = of * share + first + j;
+#pragma unroll
+            for (int r = 0; r < kMaxCluster; ++r) {  // all reads under way together
+                if (r >= ranks) continue;
+                m[j] += *cg::this_cluster().map_shared_rank(&s.hist.lo[b], r);
+                if (MASS) m[j] += (u64)*cg::this_cluster().map_shared_rank(&s.hist.hi[b], r) << 32;
+            }
+            sum += m[j];
+        }
+        before += block_scan(sum, unused);
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; ++j) {
+            if (before < target && before + m[j] >= target) { s.found[0] = (u64)(of * share + first + j); s.found[1] = before; }
+            before += m[j];
+        }
+        __syncthreads();
         const int bin = (int)s.found[0];
         const u64 above = s.found[1];
         if (threadIdx.x == 0) s.n = 0;
