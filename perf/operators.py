@@ -225,8 +225,7 @@ def _prepare_sample(case, g, dev):
     height = case["peak"] * (0.4 + 0.8 * torch.rand(B, 1, generator=g, device=dev))
     likely = torch.randint(0, V, (B, 48), generator=g, device=dev)
     fall = 0.35 * torch.arange(48, device=dev)
-    # an index that comes twice keeps the larger value (a plain scatter would leave it to chance which one)
-    logits.scatter_reduce_(1, likely, height - fall * torch.rand(B, 1, generator=g, device=dev), "amax", include_self=False)
+    logits.scatter_(1, likely, height - fall * torch.rand(B, 1, generator=g, device=dev))
     s = {"op": "sample", "logits": logits.to(DTYPES[case["dtype"]]),
          "u": torch.rand(B, generator=g, device=dev),
          "temperature": case["temperature"], "top_k": case["top_k"], "top_p": case["top_p"], "min_p": case["min_p"]}
