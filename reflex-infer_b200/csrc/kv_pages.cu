@@ -6,6 +6,11 @@
 // the bookkeeping and leave a list of copies: the layers of a model share one table, and kv_copy_pages
 // takes the caches of all of them in one launch.
 //
+// Every kernel here waits for what is ahead of it before it touches memory, and lets the kernel behind it start
+// only after that. The last kernel of a fork, a free or a compaction does not let it start early at all: it writes 32-bit
+// words (positions to copy, counts of owners) that a caller may give to attention as context lengths, and the plan kernel
+// (plan.cu) reads those before its own wait.
+//
 // Algorithmic bytes: 4 per page (counts) and 8 per table entry read and written; copies 2 * moved bytes.
 #include <cooperative_groups.h>
 
@@ -182,7 +187,6 @@ __device__ __forceinline__ void fork_entries(const ForkParams& P, const Child& c
 // (Two launches cost the host 4 us more, which is what a small fork takes.)
 constexpr int kForkCluster = 8;
 __global__ void __cluster_dims__(kForkCluster, 1, 1) __launch_bounds__(kForkThreads) kv_fork_small_kernel(const ForkParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
     const int lane = threadIdx.x & 31, warps = kForkCluster * kForkThreads / 32;
     const int64_t first = blockIdx.x * (kForkThreads / 32) + (threadIdx.x >> 5);
@@ -198,12 +202,11 @@ __global__ void __cluster_dims__(kForkCluster, 1, 1) __launch_bounds__(kForkThre
 }
 // Large ones in two.
 __global__ void __launch_bounds__(kForkThreads) kv_fork_take_kernel(const ForkParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();
     fork_take(P);
 }
 __global__ void __launch_bounds__(256) kv_fork_table_kernel(const ForkParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
     const int64_t i = blockIdx.x;
     const Child c = child_of(P, i);
@@ -216,7 +219,6 @@ __global__ void __launch_bounds__(256) kv_fork_table_kernel(const ForkParams P) 
 // once. A count that is zero already stays zero.
 __global__ void __launch_bounds__(256) kv_free_kernel(int64_t* table, int64_t bt_s, const int32_t* rows, int64_t batch,
                                                       int64_t max_blocks, int64_t num_blocks, int32_t* counts) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
     const int64_t r = rows[blockIdx.x];
     if (r < 0 || r >= batch) return;
@@ -309,7 +311,6 @@ __device__ __forceinline__ void compact_apply(const CompactParams& P, int64_t fi
 constexpr int kCompactCluster = 8;
 constexpr int64_t kSmallCompact = 1 << 15;  // pages, and table entries
 __global__ void __cluster_dims__(kCompactCluster, 1, 1) __launch_bounds__(kCompactThreads) kv_compact_small_kernel(const CompactParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
     for (int g = blockIdx.x; g < P.chunks; g += kCompactCluster) compact_count(P, g);
     cooperative_groups::this_cluster().sync();
@@ -318,17 +319,16 @@ __global__ void __cluster_dims__(kCompactCluster, 1, 1) __launch_bounds__(kCompa
     compact_apply(P, blockIdx.x * (int64_t)kCompactThreads + threadIdx.x, kCompactCluster * kCompactThreads);
 }
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_count_kernel(const CompactParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();
     compact_count(P, blockIdx.x);
 }
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_place_kernel(const CompactParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();
     compact_place(P, blockIdx.x);
 }
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_apply_kernel(const CompactParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
     compact_apply(P, blockIdx.x * (int64_t)kCompactThreads + threadIdx.x, (int64_t)gridDim.x * kCompactThreads);
 }
@@ -352,8 +352,8 @@ template <typename S> struct CopyParams {
 // under way before the first store.
 template <typename VEC, int PER, typename S>
 __global__ void __launch_bounds__(256) kv_copy_pages_kernel(const CopyParams<S> P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();
     const int lane = threadIdx.x & 31;
     int64_t pairs = P.n_pairs;
     if (P.n_moves) {

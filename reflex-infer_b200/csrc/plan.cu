@@ -59,7 +59,6 @@ plan_kernel(const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ q_
     __shared__ long long red[kPlanThreads / 32][2];
     ptx::pdl_trigger();  // the partial kernel may set itself up while the plan is computed
     const int tid = threadIdx.x;
-    for (long long i = tid; i < (long long)B * Hkv; i += kPlanThreads) pair_counter[i] = 0;
     const int per = (B + kPlanThreads - 1) / kPlanThreads;  // requests per thread, contiguous
     const int b0 = min(B, tid * per), b1 = min(B, b0 + per);
 
@@ -185,7 +184,16 @@ plan_kernel(const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ q_
     const int any_one_row = __syncthreads_or(one_row);
     if (tid == 0 && q_start) over |= ((long long)q_start[B] - q_start[0] != n_q) ? 1 : 0;
     over |= (n_items > max_items || n_rows > cap_rows) ? 1 : 0;
-    if (__syncthreads_or(over)) {
+    const bool too_large = __syncthreads_or(over);
+
+    // Up to here context_lens and q_start were read and nothing was written: that may run beside whatever is
+    // ahead in the stream, as no kernel of this library that lets its successor start early writes them. The
+    // workspace may still be in use: by the attention of the step before, when the kernel between (an append, a
+    // sampling) has let this one start, or, under another name, as a temporary of that kernel. So every
+    // store comes behind the wait.
+    ptx::pdl_wait();
+    for (long long i = tid; i < (long long)B * Hkv; i += kPlanThreads) pair_counter[i] = 0;
+    if (too_large) {
         for (long long i = tid; i <= (long long)B * Hkv; i += kPlanThreads) pair_item_begin[i] = 0;
         if (tid == 0) {
             part_first[0] = 0;
@@ -198,7 +206,6 @@ plan_kernel(const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ q_
             hdr[HdrOneRowRequests] = 0;
             hdr[HdrNumUnits] = 0;
         }
-        ptx::pdl_wait();
         return;
     }
 
@@ -253,9 +260,6 @@ plan_kernel(const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ q_
         hdr[HdrTotalRows] = (int)n_rows;
         hdr[HdrOneRowRequests] = any_one_row ? 1 : 0;
     }
-    // The plan reads nothing its predecessor wrote, but its successor (the partial kernel) does
-    // (the pool pages just appended): do not complete before the predecessor has.
-    ptx::pdl_wait();
 }
 
 int launch_plan(const RfxPagedAttentionArgs* a, const PlanLayout& L, const PlanPtrs& P, int parts_hint, int item_cost,

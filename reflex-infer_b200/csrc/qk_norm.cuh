@@ -125,8 +125,8 @@ template <int V> __device__ __forceinline__ void mul_v(const float (&x)[V], cons
 // LANES: the lanes of a row where a row is exactly that many pieces, 0 where lanes stay idle or take several.
 template <typename T, typename TT, int V, int NP, int LANES, bool INTER, int MODE>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormParams P) {
-    ptx::pdl_trigger();  // the kernel behind this one waits for this one's end before it reads anything
     ptx::pdl_wait();
+    ptx::pdl_trigger();  // behind the wait: what starts now finds everything ahead of this kernel complete
     const int lane = threadIdx.x & 31;
     const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
     const int64_t n = warp / P.splits;

@@ -1079,8 +1079,8 @@ template <typename T> struct Row {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams P) {
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();
     extern __shared__ __align__(16) unsigned char stage[];
     __shared__ Shared shared;
     auto cluster = cg::this_cluster();
