@@ -271,7 +271,7 @@ template <typename T> struct Row {
     __device__ __forceinline__ void set_top(float v) {
         top = v;
         top_wide = (double)fminf(v, -kLowest);
-        zero_below = v == INFINITY ? INFINITY : fmaxf(kLowest, (float)(top_wide - 32.0 * (shift + 2) / scale));
+        zero_below = v == INFINITY ? INFINITY : fmaxf(kLowest, __double2float_ru(top_wide - 32.0 * (shift + 2) / scale));
         cut_value = zero_below;
     }
     // A chunk that reaches over an end of the slice (the first or the last one), element by element.
