@@ -342,7 +342,10 @@ int rfx_online_softmax(const RfxSoftmaxArgs* a);
  * temperature <= 0 or NaN: the lowest index of the largest logit (above 0 it counts as 1e-20 at least). A row with nothing but -inf (or NaN) gives
  * -1; with +inf among its logits those share the mass. Every setting is a device array [batch], or with a
  * NULL pointer one number for all rows. Weights are computed to 2^-39 of themselves and summed as whole multiples
- * of 2^-S of the largest, S = min(50, 62 - log2 vocab): the result depends on nothing but the arguments. vocab <= 2^24. */
+ * of 2^-S of the largest: the result depends on nothing but the arguments. S = min(50, 63 - log2 M) with M the top_k or vocab
+ * logits that can weigh anything, up to M = 2^18, beyond that as much as keeps the row's total below 2^63, at most 50; a
+ * running sum is off by no more than M 2^-(S+1) of the largest weight, 2^-30 at 131072 tokens and 2^-27 of the total at the
+ * most. vocab <= 2^24. */
 typedef struct {
     const void* logits;          /* [batch, vocab], row stride below, last dim contiguous */
     const float* uniform;        /* [batch], in [0, 1) */

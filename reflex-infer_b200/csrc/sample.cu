@@ -6,9 +6,13 @@
 //   the token is the lowest index whose running sum of kept weights, in index order, exceeds u * their sum.
 //
 // The answer hangs on which side of a border a sum lies, so sums must not depend on the order in which
-// threads or CTAs run: a weight is computed in 64 bits to 2^-39 of itself, rounded to a whole multiple of 2^-S with
-// S = min(50, 62 - log2 V), and added up as a 64-bit integer. Such sums are exact in any order; what a weight loses is far
-// below the distance of two borders (131072 tokens: a border in 3e-7 rows is that near the number drawn).
+// threads or CTAs run: a weight is computed in 64 bits to 2^-39 of itself, rounded to a whole multiple of 2^-S of the
+// largest, and added up as a 64-bit integer. Such sums are exact in any order. With M logits that can weigh anything (M = top-k, or
+// V) all of them may weigh the same, so S = min(50, 63 - log2 M), log2 rounded up, keeps any sum below 2^63. Equal logits all
+// round the same way, so a sum may be off by M 2^-(S+1) of the largest weight: 2^-38 up to M = 2^13, 2^-30 at 2^17, 2^-28
+// at 2^18. Beyond that such a bound would reach the 2^-24 between two uniform numbers (2^24 logits, all but one 27 below that
+// one: a mass of 3e-5 would be lost). There a pass adds up the row at that S first, and S is raised as far as this sum allows
+// (see sharpen()): then a sum is off by 2^-27 of the total at most.
 //
 // A cluster of up to 8 CTAs takes a row, each a slice of it (one CTA a row in large batches). Two ways to the
 // answer, by the row's settings:
@@ -53,6 +57,8 @@ constexpr int kBatch = 4;                 // 16-byte chunks a thread has under w
 constexpr size_t kStageTwo = 72 * 1024;   // slice that lets two CTAs share an SM
 constexpr size_t kStageMax = 180 * 1024;  // largest slice kept in shared memory
 constexpr int kParts = 8;                 // of a warp's range in the draw
+constexpr int kShift = 50;                // the largest S: a weight and 2^52 have to fit a double
+constexpr int kFewWeights = 1 << 18;      // logits that can weigh anything, up to which S follows from their number alone
 constexpr float kLowest = -3.402823466e38f;
 
 enum { kAllRows = 0, kListRows = 1, kOtherRows = 2 };
@@ -65,8 +71,7 @@ struct SampleParams {
     float temperature0, top_p0, min_p0;
     int32_t top_k0;
     int vocab, slice;  // slice: logits per CTA, a multiple of 8
-    int shift;         // S: weights are multiples of 2^-S
-    double power[32];  // 2^(S + i/32), with i * 2^15 taken off the upper word
+    double power[32];  // 2^(kShift + i/32), with i * 2^15 taken off the upper word
     int staged;        // general rows keep their slice in shared memory
     int rows;          // which rows this launch takes
 };
@@ -85,7 +90,7 @@ struct __align__(16) Shared {
     u64 slot[2][kMaxCluster];  // words of the other CTAs, written by them
     u64 shares[2][kMaxCluster][kMaxCluster];  // [top-k, top-p][CTA][share of the bins]: what that CTA's logits add to it
     u64 found[3];              // a bin and the sum before it; what one CTA tells all, a cut
-    double power[32];          // as in SampleParams
+    double power[32];          // as in SampleParams, for the row's S
     uint32_t picked[3];        // of select(): the bound, the largest key, n before it
     int n;                     // entries that want to be in `list`
 };
@@ -273,6 +278,30 @@ template <typename T> struct Row {
         top_wide = (double)fminf(v, -kLowest);
         zero_below = v == INFINITY ? INFINITY : fmaxf(kLowest, __double2float_ru(top_wide - 32.0 * (shift + 2) / scale));
         cut_value = zero_below;
+    }
+    // S of a row, see the head of this file. `some`: logits that can weigh anything
+    __device__ __forceinline__ static int shift_of(int some) { return min(kShift, 63 - (32 - __clz(some - 1))); }
+    // Raises S by the steps that the sum of the row's masses leaves room for. With x that sum and one more per logit (rounding takes half
+    // a unit at most), the sum at S + d is at most x 2^d; d = clz(x) - 1 keeps that below 2^63. The sum is over the whole row, before any cut, so
+    // what is kept later has room too.
+    __device__ __forceinline__ void sharpen() {
+        u64 sum = 0;
+        each_chunk([&](const Chunk<T>& c, int) {
+            if (!(c.most() >= zero_below)) return;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                int unused;
+                const double w = mass_of(c.raw_at(e), unused);
+                sum += c.raw_at(e) >= zero_below ? low52(w) : 0;
+            }
+        });
+        sum = cluster_sum(sum);
+        const int more = min(kShift - shift, max(0, __clzll((long long)(sum + (u64)vocab)) - 1));
+        if (threadIdx.x < 32)  // (nobody looks for a weight between the barriers of the sum and this one)
+            s.power[threadIdx.x] = __hiloint2double(__double2hiint(s.power[threadIdx.x]) + (more << 20), __double2loint(s.power[threadIdx.x]));
+        __syncthreads();
+        shift += more;
+        set_top(top);
     }
     // A chunk that reaches over an end of the slice (the first or the last one), element by element.
     __device__ __forceinline__ Chunk<T> load_edge(int j) const {
@@ -1092,7 +1121,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const T* row = (const T*)P.logits + b * P.row_stride;
     const int lo = min(P.vocab, rank * P.slice), hi = min(P.vocab, lo + P.slice);
     const int phase = (int)(((uintptr_t)(row + lo) & 15) / sizeof(T));
-    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0, P.vocab, P.shift, false};
+    R r{row, (T*)stage, lo, hi, lo - phase, lo < hi ? (hi - lo + phase + N - 1) / N : 0, shared, rank, ranks, 0, P.vocab, 0, false};
 
     const float temperature = P.temperature ? P.temperature[b] : P.temperature0;
     const float p = P.top_p ? P.top_p[b] : P.top_p0, min_p = P.min_p ? P.min_p[b] : P.min_p0;
@@ -1110,11 +1139,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const double t = fmax((double)temperature, 1e-20);
     r.scale = fmax(32.0 * 1.4426950408889634 / t, 1e-300);  // at T = inf every finite logit weighs 1
     r.cut_index = 0x7fffffff;
-    if (threadIdx.x < 32) shared.power[threadIdx.x] = P.power[threadIdx.x];
+    const bool few = k <= kFewWeights;
+    r.shift = R::shift_of(few ? k : P.vocab);
+    if (threadIdx.x < 32) {
+        const double w = P.power[threadIdx.x];
+        shared.power[threadIdx.x] = __hiloint2double(__double2hiint(w) - ((kShift - r.shift) << 20), __double2loint(w));
+    }
     cluster.barrier_wait(std::move(started));
 
     if (by_list) {
-        r.stream(k, (float)((P.shift + 2) * 0.6931471805599454 * t));  // weights end before that far below the largest
+        r.stream(k, (float)((r.shift + 2) * 0.6931471805599454 * t));  // weights end before that far below the largest
         const int n = r.top == -INFINITY ? 0 : r.collect();
         if (r.top > -INFINITY && n <= kCap) {
             // rank 0 has pulled the lists: the others may leave
@@ -1132,6 +1166,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
         return;
     }
     if (greedy) return r.greedy(token);
+    if (!few) r.sharpen();
     if (k < P.vocab) r.template cut<false>(k, 0.f);
     if (p < 1.f) r.template cut<true>(0, p);
     r.draw(u, min_p, token);
@@ -1177,11 +1212,8 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
     P.top_k = a->top_k; P.tokens = a->tokens; P.row_stride = a->row_stride;
     P.temperature0 = a->temperature_all; P.top_p0 = a->top_p_all; P.min_p0 = a->min_p_all; P.top_k0 = a->top_k_all;
     P.vocab = (int)a->vocab;
-    int log2v = 0;
-    while ((1ll << log2v) < a->vocab) ++log2v;
-    P.shift = 62 - log2v < 50 ? 62 - log2v : 50;
     for (int i = 0; i < 32; ++i) {
-        const double w = ldexp(exp2(i / 32.0), P.shift);
+        const double w = ldexp(exp2(i / 32.0), kShift);
         uint64_t bits;
         memcpy(&bits, &w, 8);
         bits -= (uint64_t)i << 47;
