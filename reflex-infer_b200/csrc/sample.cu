@@ -18,8 +18,8 @@
 // answer, by the row's settings:
 //   list     (top-k up to 512) The logits stream through registers once. Every thread keeps the largest of two groups
 //            of its own; the k-th largest of the CTA's 1024 group maxima bounds the k-th largest logit from below, and
-//            what reaches the bound, renewed whenever the logits seen have doubled, goes to a list in shared
-//            memory. About 1.3 k logits are left in the end; one CTA ranks them, and has the kept set in hand.
+//            what reaches the bound, renewed whenever four times as many logits have been seen (twice as many
+//            where k is above 227), goes to a list in shared memory. About 1.3 k logits are left in the end; one CTA ranks them, and has the kept set in hand.
 //   general  The slice stays in shared memory (or is read again from L2). A histogram over max - l (counts for top-k,
 //            masses for top-p) names the bin with the border, the logits of that bin are ranked, and a pass in index
 //            order adds up what is kept. Without top-k and top-p only that pass is left.
@@ -879,8 +879,7 @@ template <typename T> struct Row {
             const float d = top - value_of((uint32_t)(e >> 32));
             return d > 0.f ? min(kBins - 1, (int)(fminf(d, 3.4e38f) * per_unit)) : 0;
         });
-        if (min(n, k) <= kThreads) finish_sorted<1>(min(n, k), p, least, u, token);
-        else finish_sorted<kCap / kThreads>(min(n, k), p, least, u, token);
+        finish_sorted(min(n, k), p, least, u, token);
     }
     // The smallest key of list[0, n), over the whole CTA, in every lane.
     __device__ __forceinline__ uint32_t lowest_key(int n) {
@@ -892,66 +891,31 @@ template <typename T> struct Row {
         __syncthreads();
         return __reduce_min_sync(0xffffffffu, (uint32_t)s.part[threadIdx.x & (kWarps - 1)]);
     }
-    // The rest over a sorted list of at most PER * kThreads entries, PER neighbours a thread.
-    template <int PER> __device__ __forceinline__ void finish_sorted(int n, float p, u64 least, float u, int64_t* token) {
-        u64 m[PER], e[PER], sum = 0, total;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            e[j] = i < n ? s.list[i] : 0;
-            m[j] = i < n ? mass((uint32_t)(e[j] >> 32)) : 0;
-            sum += m[j];
-        }
-        u64 before = block_scan(sum, total);
-        const u64 target = p < 1.f ? target_of(p, total) : ~0ull;
-        int stay = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const bool in = e[j] && before < target && m[j] >= least;
-            before += m[j];
-            if (!in) m[j] = 0;
-            stay += in;
-        }
-        const int kept_n = (int)block_sum((u64)stay);  // a prefix of the list: weights only fall
+    // The rest over the first n <= kListK entries of a sorted list, one a thread.
+    __device__ __forceinline__ void finish_sorted(int n, float p, u64 least, float u, int64_t* token) {
+        static_assert(kListK <= kThreads, "an entry a thread");
+        const int i = threadIdx.x;
+        u64 total, e = i < n ? s.list[i] : 0, m = i < n ? mass((uint32_t)(e >> 32)) : 0;
+        const u64 before = block_scan(m, total);
+        const bool in = e && before < (p < 1.f ? target_of(p, total) : ~0ull) && m >= least;
+        if (!in) m = 0;
+        const int kept_n = (int)block_sum((u64)in);  // a prefix of the list: weights only fall
         if (kept_n <= kPairs) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const int i = threadIdx.x * PER + j;
-                if (i < kept_n) s.pair[i] = Entry{e[j] << 32, m[j]};  // falling in ~index: rising in index
-            }
+            if (i < kept_n) s.pair[i] = Entry{e << 32, m};  // falling in ~index: rising in index
             __syncthreads();
             return draw_pairs(kept_n, u, token);
         }
         // in index order: entries (index, place), with their weights beside them
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            if (i < kept_n) s.list[i] = e[j] << 32 | (u64)i;
-        }
+        if (i < kept_n) s.list[i] = e << 32 | (u64)i;
         const float per_index = (float)(kBins - 1) / (float)vocab;
         sort_by_bins(s, kept_n, [&](u64 x) { return (int)((float)(0xffffffffu - (uint32_t)(x >> 32)) * per_index); });
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            if (i < kept_n) s.weight[i] = m[j];
-        }
+        if (i < kept_n) s.weight[i] = m;
         __syncthreads();
-        sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int i = threadIdx.x * PER + j;
-            e[j] = i < kept_n ? s.list[i] : 0;
-            m[j] = i < kept_n ? s.weight[(uint32_t)e[j]] : 0;
-            sum += m[j];
-        }
-        u64 at = block_scan(sum, total);
-        const u64 x = drawn(u, total);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            if (x >= at && x < at + m[j]) *token = (int64_t)(0xffffffffu - (uint32_t)(e[j] >> 32));
-            at += m[j];
-        }
+        e = i < kept_n ? s.list[i] : 0;
+        m = i < kept_n ? s.weight[(uint32_t)e] : 0;
+        const u64 at = block_scan(m, total), x = drawn(u, total);
+        if (x >= at && x < at + m) *token = (int64_t)(0xffffffffu - (uint32_t)(e >> 32));
     }
     // The draw among pair[0, n): keys that fall as the index rises, and masses. Entry i belongs to thread i.
     __device__ __forceinline__ void draw_pairs(int n, float u, int64_t* token) {

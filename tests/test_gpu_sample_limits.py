@@ -104,3 +104,39 @@ def test_long_rows_in_batches_and_with_top_k(native):
     assert sample_tokens(gx, gu, top_k=gk, top_p=gp).tolist() == want
     for b in (0, 1, 2, 3, 5, 11):
         assert sample_tokens(gx[b:b + 1], gu[b:b + 1], top_k=int(top_k[b]), top_p=float(top_p[b])).tolist() == want[b:b + 1]
+
+
+@pytest.mark.parametrize("V,B", [(600, 7), (5000, 9), (40001, 4), (131072, 3)])
+def test_top_k_up_to_the_longest_list(native, V, B):
+    """Top-k rows with more kept than are ranked by comparing pairs, up to the 512 that the list way takes and one beyond."""
+    g = torch.Generator().manual_seed(V)
+    x = 2 * torch.randn(B, V, generator=g)
+    x[0] = torch.round(x[0])
+    x[1, V // 2:] = -math.inf
+    u = torch.rand(B, generator=g)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        for k in (128, 129, 227, 228, 300, 511, 512, 513):
+            for kw in (dict(), dict(top_p=0.95), dict(top_p=0.6, min_p=0.02), dict(temperature=30.0), dict(min_p=1e-3, temperature=0.5)):
+                assert sample_tokens(y.to(DEV), u.to(DEV), top_k=k, **kw).tolist() == sample_oracle.tokens(y, u, top_k=k, **kw), (k, kw)
+
+
+@pytest.mark.parametrize("V", [20000, 60000, 128000])
+def test_rows_masked_but_for_a_stretch(native, V):
+    """Rows that several CTAs take, with whole slices of nothing but -inf: the few CTAs with logits give the answer."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.full((6, V), -math.inf)
+    x[0, :V // 8] = 2 * torch.randn(V // 8, generator=g)
+    x[1, -V // 5:] = 2 * torch.randn(x[1, -V // 5:].shape, generator=g)
+    x[2, V // 2:V // 2 + 30] = torch.randn(30, generator=g)
+    x[3, ::997] = 1.5
+    x[4, V - 1] = -4.0
+    x[5] = torch.finfo(torch.float32).min
+    x[5, 100:V // 3] = 2 * torch.randn(V // 3 - 100, generator=g)
+    u = torch.tensor([0.1, 0.9, 0.5, 0.99, 0.3, 0.7])
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        for kw in (dict(), dict(top_k=40), dict(top_k=300, top_p=0.9), dict(top_p=0.9), dict(top_k=2000), dict(min_p=0.1), dict(temperature=0.0)):
+            want = sample_oracle.tokens(y, u, **kw)
+            assert sample_tokens(y.to(DEV), u.to(DEV), **kw).tolist() == want, kw
+            assert sample_tokens(y[:1].to(DEV), u[:1].to(DEV), **kw).tolist() == want[:1], kw
