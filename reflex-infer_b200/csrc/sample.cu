@@ -1070,7 +1070,9 @@ template <typename T> struct Row {
     }
 };
 
-template <typename T>
+// LONG: rows of more than kFewWeights logits. A kernel of its own: with the pass that they need in it the others took up to 4 %
+// longer (256 x 131072 fp32: no cut 88.6 us and 85.4, top-p 191 and 187).
+template <typename T, bool LONG>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams P) {
     ptx::pdl_wait();
     ptx::pdl_trigger();
@@ -1103,7 +1105,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams 
     const double t = fmax((double)temperature, 1e-20);
     r.scale = fmax(32.0 * 1.4426950408889634 / t, 1e-300);  // at T = inf every finite logit weighs 1
     r.cut_index = 0x7fffffff;
-    const bool few = k <= kFewWeights;
+    const bool few = !LONG || k <= kFewWeights;
     r.shift = R::shift_of(few ? k : P.vocab);
     if (threadIdx.x < 32) {
         const double w = P.power[threadIdx.x];
@@ -1212,17 +1214,21 @@ extern "C" int rfx_sample_tokens(const RfxSampleArgs* a) {
         cfg.numAttrs = 2;
         le = cudaLaunchKernelEx(&cfg, kern, P);
     };
-    RFX_DISPATCH_DTYPE(a->dtype, T, {
-        static PerDeviceOnce once;
+    auto launch_all = [&](auto kern, PerDeviceOnce& once) {
         // Where top-k is given row by row, in batches that fill the GPU with one CTA a row, list rows want one CTA and the others
         // several: a launch for each kind (256 x 131072 fp32, lists alone: 39 us, in one launch of one CTA a row 34, of
         // four 60; mixed: 122, 166 and 105).
         if (a->top_k && a->batch >= sms && C_others > 1) {
-            launch(sample_kernel<T>, once, C_lists, kListRows);
-            if (le == cudaSuccess) launch(sample_kernel<T>, once, C_others, kOtherRows);
+            launch(kern, once, C_lists, kListRows);
+            if (le == cudaSuccess) launch(kern, once, C_others, kOtherRows);
         } else {
-            launch(sample_kernel<T>, once, all_lists ? C_lists : C_others, kAllRows);
+            launch(kern, once, all_lists ? C_lists : C_others, kAllRows);
         }
+    };
+    RFX_DISPATCH_DTYPE(a->dtype, T, {
+        static PerDeviceOnce once, once_long;
+        if (a->vocab > kFewWeights) launch_all(sample_kernel<T, true>, once_long);
+        else launch_all(sample_kernel<T, false>, once);
     });
     if (le != cudaSuccess) { cudaGetLastError(); return fail(RFX_CUDA_ERROR, "%s: %s", name, cudaGetErrorString(le)); }
     return check_launch(name);
