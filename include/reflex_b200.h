@@ -132,8 +132,11 @@ int rfx_kv_paged_lookup(const RfxKvLookupArgs* a);
  * take pages in order. child_table[i] gets the row, -1 behind it. A child for which no page is left has
  * src_pages[i] >= 0 and dst_pages[i] = -1; it, and one whose parent is no row, gets a row of -1 and holds
  * nothing. A table entry outside the pool is passed on as it is. Lengths are taken as at most
- * max_blocks * block_size. No page is both source and destination: a page that a child copies from is not
- * handed out, and if its count was 0 it becomes 1. */
+ * max_blocks * block_size. The counts have to be true: every page that a parent's row names within its length has a
+ * count of 1 at least, and then no page of any row is handed out. A count of 0 says that the page is free, and a whole page with
+ * that count may be given to another child of the same call, whose copy then overwrites it. One thing holds even so, since the
+ * copies run side by side: no page is both source and destination; a part-filled page that a child copies from is not handed
+ * out, and if its count was 0 it becomes 1. */
 typedef struct {
     const int64_t* block_table;  /* [batch, max_blocks], row stride bt_stride_b */
     const int32_t* context_lens; /* [batch] */

@@ -111,7 +111,8 @@ __device__ __forceinline__ void fork_take(const ForkParams& P) {
     __shared__ int64_t next_from;
     const bool aligned = ((uintptr_t)P.counts & 15) == 0;
     int64_t from = 0;
-    // No page that a child copies from is handed out, even if its count says that it is free.
+    // No page that a child copies from is handed out, even if its count says that it is free: the copies run side by side. (Whole
+    // pages that are shared are not looked at here; that they count 1 at least is the caller's part.)
     Child mine_first = {-1, 0, 0, -1};
     for (int64_t i = threadIdx.x; i < P.n; i += kForkThreads) {
         const Child c = child_of(P, i);

@@ -203,8 +203,12 @@ def kv_fork(
     appended. ``child_table`` is ``[n, max_blocks]`` int64, -1 behind the child's pages. Children take free
     pages in order; one for which none is left has ``moves.src >= 0`` and ``moves.dst < 0``, and it (and one
     whose parent is no row) gets a row of -1 and holds nothing. A parent may have any number of children;
-    it keeps its own pages until ``kv_free``. A page that a child copies from is never handed out (a count of
-    0 there, which says that nobody holds it, becomes 1).
+    it keeps its own pages until ``kv_free``.
+
+    ``ref_counts`` has to be true: every page that a parent's row names within its length counts 1 at least, and then no
+    page of any row is handed out. A page that counts 0 is free: a whole one that a row names all the same may become another
+    child's own page and be overwritten by its copy. Only the part-filled page that a child copies from is never handed
+    out, whatever its count (0 becomes 1), so the copies of one call cannot meet.
     """
     N.check_backend(backend)
     name = "kv_fork"
