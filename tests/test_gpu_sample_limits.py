@@ -140,3 +140,15 @@ def test_rows_masked_but_for_a_stretch(native, V):
             want = sample_oracle.tokens(y, u, **kw)
             assert sample_tokens(y.to(DEV), u.to(DEV), **kw).tolist() == want, kw
             assert sample_tokens(y[:1].to(DEV), u[:1].to(DEV), **kw).tolist() == want[:1], kw
+
+
+def test_long_rows_in_a_launch_for_each_kind(native):
+    """As many long rows as make top-k row by row two launches: the tokens that the rows have in small batches."""
+    B, V = 160, (1 << 18) + 3
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = (2 * torch.randn(B, V, generator=g, device=DEV)).to(torch.bfloat16)
+    u = torch.rand(B, generator=g, device=DEV)
+    top_k = torch.tensor([30, 0, 5000, V - 1, 512, (1 << 18) + 1], device=DEV)[torch.arange(B, device=DEV) % 6].to(torch.int32)
+    whole = sample_tokens(x, u, top_k=top_k, top_p=0.95)
+    for b in range(0, B, 8):
+        assert torch.equal(sample_tokens(x[b:b + 8], u[b:b + 8], top_k=top_k[b:b + 8], top_p=0.95), whole[b:b + 8])
