@@ -190,7 +190,8 @@ plan_kernel(const int32_t* __restrict__ ctx_lens, const int32_t* __restrict__ q_
     // ahead in the stream, as no kernel of this library that lets its successor start early writes them. The
     // workspace may still be in use: by the attention of the step before, when the kernel between (an append, a
     // sampling) has let this one start, or, under another name, as a temporary of that kernel. So every
-    // store comes behind the wait.
+    // store comes behind the wait. (A step of 32 requests, 16/2 heads: 52.7 to 53.5 us; with the stores beside rope_append as well
+    // 52.4 to 52.8.)
     ptx::pdl_wait();
     for (long long i = tid; i < (long long)B * Hkv; i += kPlanThreads) pair_counter[i] = 0;
     if (too_large) {
