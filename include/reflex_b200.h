@@ -416,7 +416,10 @@ typedef struct {
     const void* k_cache;         /* [num_blocks, H_kv, block_size, D] contiguous */
     const void* v_cache;
     const int64_t* block_table;  /* [B, max_blocks] */
-    const int32_t* context_lens; /* [B] keys per request, new tokens included */
+    const int32_t* context_lens; /* [B] keys per request, new tokens included. The plan reads this and q_start as soon
+                                  * as it may start: where a kernel of the caller's own that lets its successor start early
+                                  * (griddepcontrol.launch_dependents) writes them, put an ordinary launch, a copy or an
+                                  * event in between. No kernel of this library that does so writes such words. */
     const int32_t* q_start;      /* [B+1] or NULL (decode: row b belongs to request b) */
     /* optional RoPE fused into the Q load (rows rope_positions[n] of the tables) */
     const void* rope_cos;        /* [table_rows, D] activation dtype, or NULL */

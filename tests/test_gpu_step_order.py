@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kernels.attention import PagedWorkspace, int8_pool, paged_attention, paged_decode_step
+from kernels.attention import PagedAttentionCall, PagedWorkspace, int8_pool, paged_attention, paged_decode_step, qk_norm_rope_append
 from kernels.kv_cache import kv_compact, kv_copy_pages, kv_fork, kv_free
 from kernels.rope import build_rope_tables
 from kernels.softmax import online_softmax, sample_tokens
@@ -103,6 +103,17 @@ def test_steps_of_one_batch(native):
 def test_steps_with_arguments_that_are_cast(native):
     """64-bit positions and lengths and 32-bit slots: the calls make temporaries, whose memory the next call may get."""
     _run(_batches(128, torch.bfloat16, False, torch.int64), [0, 1] * 6, lambda b, ws, o: b.step(None, o) if o is not None else b.step(ws), PagedWorkspace(DEV))
+
+
+def test_steps_on_the_built_in_scratch(native):
+    """The same with the scratch that is part of the library in place of a workspace: every call plans there afresh."""
+    batches = _batches(128, torch.bfloat16, False)
+
+    def call(b, ws, o):
+        q = qk_norm_rope_append(b.q, b.k, b.v, b.kc, b.vc, b.slots, b.pos, b.cos, b.sin, b.wq, b.wk)
+        return PagedAttentionCall(q, b.kc, b.vc, b.table, b.lens, out=o, max_q_len=1).run_static()
+
+    _run(batches, [0, 1, 0, 1, 1, 0, 0, 1], call, PagedWorkspace(DEV))
 
 
 @pytest.mark.parametrize("between", ["sample", "pages", "softmax", "nothing"])
